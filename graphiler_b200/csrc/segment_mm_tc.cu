@@ -22,6 +22,7 @@
 #include <cuda.h>
 
 #include "common.cuh"
+#include "tc_gemm.cuh"
 
 namespace gphl {
 
@@ -600,7 +601,7 @@ extern "C" int gphl_debug_wait_selftest(int32_t polls, void *stream) {
 extern "C" int gphl_debug_reset_wait_timeouts(void) {
   const int zero = 0;
   GPHL_CUDA(cudaMemcpyToSymbol(gphl::g_tc_wait_timeouts, &zero, sizeof(int)));
-  return GPHL_OK;
+  return gphl::gemm_reset_wait_timeouts();
 }
 
 // Number of barrier waits that ran out in tensor-core kernels since the library was loaded
@@ -608,5 +609,8 @@ extern "C" int gphl_debug_reset_wait_timeouts(void) {
 extern "C" int gphl_tc_wait_timeouts(int *count) {
   GPHL_REQUIRE(count != nullptr, "null pointer argument");
   GPHL_CUDA(cudaMemcpyFromSymbol(count, g_tc_wait_timeouts, sizeof(int)));
-  return GPHL_OK;
+  int dense = 0;
+  const int rc = gemm_wait_timeouts(&dense);
+  *count += dense;
+  return rc;
 }

@@ -1,0 +1,61 @@
+// The tensor-core product behind the dense operators (tc_gemm.cu): what a launch is told, and its host entry.
+#pragma once
+
+#include <cuda.h>
+
+#include "common.cuh"
+
+namespace gphl {
+
+// A matrix in device memory as the product reads it: `rows` x `cols`, cols contiguous, `ld` elements from row to row.
+struct Matrix {
+  const void *p;
+  int64_t rows, cols, ld;
+};
+
+enum Activation { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
+
+// out[i, j] = sum_k A[i, k] B[j, k] for i < m, j < n, in fp32.
+//   a[0..1], b[0..1]   an operand that is stored with k contiguous ("K-major": rows are i or j), or with i / j contiguous (a_mn / b_mn:
+//                      rows are k; 16-bit types only)
+//   dual               NONE: a[0], b[0].  CONCAT: k runs over (a[0], b[0]) and then (a[1], b[1]).  BATCH: two products into out[0], out[1].
+//                      GATED: g = A b[0]^T, u = A b[1]^T, out = act(g) * u
+//   typed              rows are grouped by type: rows [ptr[t], ptr[t+1]) use rows [t n, (t+1) n) of b
+// e4m3 operands (fp8) are K-major and carry scales: A one per (row, block of 128 k), B one per (block of 128 j, block of 128 k).
+enum Dual { DUAL_NONE, DUAL_CONCAT, DUAL_BATCH, DUAL_GATED };
+struct GemmCall {
+  int in_type = GPHL_BF16;              // GPHL_BF16 / GPHL_F16; ignored when fp8
+  bool fp8 = false, a_mn = false, b_mn = false;
+  Dual dual = DUAL_NONE;
+  int64_t m = 0, n = 0, k = 0;          // k: of one pair of operands
+  Matrix a[2] = {}, b[2] = {};
+  const int32_t *ptr = nullptr;
+  int64_t types = 1;
+  const float *a_scale = nullptr, *b_scale[2] = {};
+  int64_t a_scale_row = 0, a_scale_block = 0;      // strides of a_scale
+  int act = ACT_SILU;
+  void *out[2] = {};
+  int64_t ld_out = 0;
+  int out_type = GPHL_BF16;
+  float *g = nullptr, *u = nullptr;     // GATED: also stored, m x n with row stride ld_gu
+  int64_t ld_gu = 0;
+  uint8_t *q = nullptr;                 // GATED: out as e4m3 codes (row stride ld_out) and scales (block * q_scale_stride + row)
+  float *q_scale = nullptr;
+  int64_t q_scale_stride = 0;
+  void *workspace = nullptr;            // gemm_workspace_bytes() of the same call
+};
+
+int64_t gemm_workspace_bytes(const GemmCall &c);
+int gemm(const GemmCall &c, const char *what, cudaStream_t stream);
+int gemm_wait_timeouts(int *count);
+int gemm_reset_wait_timeouts();
+
+#ifdef __CUDACC__
+__device__ __forceinline__ float activate(float g, int act) {
+  if (act == ACT_SILU) return __fdividef(g, 1.f + __expf(-g));
+  if (act == ACT_GELU) return 0.5f * g * (1.f + erff(g * 0.70710678118654752f));
+  return g > 0.f ? g : 0.f * g;                    // a NaN stays one
+}
+#endif
+
+}  // namespace gphl

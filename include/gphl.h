@@ -38,6 +38,15 @@ extern "C" {
 #define GPHL_ERR_UNSUPPORTED (-3)      /* shape outside what the kernels cover             */
 #define GPHL_ERR_TOO_LARGE (-4)        /* exceeds a stated fixed capacity                   */
 
+/* Element types of the dense operators (rms_norm, gated, fp8 products). */
+#define GPHL_F32 0
+#define GPHL_BF16 1
+#define GPHL_F16 2
+/* Activations of the gated feed-forward. */
+#define GPHL_ACT_SILU 0
+#define GPHL_ACT_GELU 1                /* g * Phi(g), the exact form                        */
+#define GPHL_ACT_RELU 2
+
 /* Message of the calling thread's last failed call ("" if none). */
 const char *gphl_last_error(void);
 /* Library version, (major << 16) | minor. */
@@ -281,6 +290,73 @@ int gphl_tc_wait_timeouts(int *count);
  * polls (<= 2^20), on a barrier nothing completes; it must return and raise the counter above by one. */
 int gphl_debug_wait_selftest(int32_t polls, void *stream);
 int gphl_debug_reset_wait_timeouts(void); /* sets the counter back to 0 (synchronises) */
+
+/* ---- dense operators of a transformer block on node rows --------------------------------------
+ *
+ * 8-bit rows ("codes"): e4m3 values with one fp32 scale per row and block of 128 columns, scale (row, b) at
+ * scales[row * scale_row_stride + b * scale_block_stride]; code rows start on 16-byte boundaries.  The quantisers write
+ * powers of two (the smallest 2^e >= 2^-126 with the block's largest finite magnitude <= 448 * 2^e), code rows padded with zeros to
+ * q_stride = n rounded up to 16, and scale (row, b) at b * scale_stride + row; a non-finite value becomes the NaN code.  The product
+ * takes any scales.  8-bit weights: w (n_types, n, k) codes, k contiguous and padded to a multiple of 16, with one scale per
+ * 128 x 128 values, (n_types, ceil(n / 128), ceil(k / 128)) contiguous.
+ */
+
+/* r = round(x + residual) in the rows' type (r = x without a residual; then r may be NULL), y = r * rstd * w with
+ * rstd = 1 / sqrt(mean(r^2) + eps).  (m, n) row-major, m rows < 2^31; w: n values of the rows' type or fp32.  rstd (m, may be NULL) is
+ * kept for the backward pass.  y may be x, r may be x or residual. */
+int gphl_rms_norm(int32_t dtype, int64_t m, int64_t n, const void *x, const void *residual, const void *w, int32_t w_dtype, float eps,
+                  void *y, void *r, float *rstd, void *stream);
+/* The same with y as codes: correctly rounded from the normalised value. */
+int gphl_rms_norm_fp8(int32_t dtype, int64_t m, int64_t n, const void *x, const void *residual, const void *w, int32_t w_dtype, float eps,
+                      void *q, int64_t q_stride, float *scales, int64_t scale_stride, void *r, void *stream);
+/* dx = dr + rstd (g - xhat mean(g xhat)) with g = dy w, xhat = r rstd (dr may be NULL); dw = sum of dy xhat over the rows, in w's type,
+ * summed in a fixed order.  `workspace`: gphl_rms_norm_grad_workspace_bytes.  dx may be dy or dr. */
+int64_t gphl_rms_norm_grad_workspace_bytes(int32_t dtype, int64_t m, int64_t n);
+int gphl_rms_norm_grad(int32_t dtype, int64_t m, int64_t n, const void *r, const void *w, int32_t w_dtype, const float *rstd, const void *dy,
+                       const void *dr, void *dx, void *dw, void *workspace, void *stream);
+
+/* Codes of the rows of x (m, n). */
+int gphl_quantize_fp8(int32_t dtype, int64_t m, int64_t n, const void *x, void *q, int64_t q_stride, float *scales, int64_t scale_stride,
+                      void *stream);
+/* Codes of the weights w (n_types, k, n) as segment_mm takes them, transposed to (n_types, n, k) with rows of k_stride = k rounded up
+ * to 16, and their scales. */
+int gphl_quantize_fp8_weight(int32_t dtype, int64_t n_types, int64_t k, int64_t n, const void *w, void *q, int64_t k_stride, float *scales,
+                             void *stream);
+/* y (m, n) = code value * scale, in `dtype`; q_stride: bytes from row to row. */
+int gphl_dequantize_fp8(int32_t dtype, int64_t m, int64_t n, const void *q, int64_t q_stride, const float *scales, int64_t scale_row_stride,
+                        int64_t scale_block_stride, void *y, void *stream);
+
+/* Rows of 16-bit values (m, n), contiguous, copied to rows 16-byte aligned (n_pad = n rounded up to 8; the padding is not written):
+ * the products below read their 16-bit operands in rows that start on 16-byte boundaries. */
+int gphl_pad_rows_16(int64_t m, int64_t n, const void *x, void *y, void *stream);
+
+/* Typed product of codes: y[i, :] = x[i, :] @ w[t]^T for the rows i of type t, type_pointer (n_types + 1) int32 as in segment_mm or
+ * NULL (one type, all rows).  Sums of a block of 128 are scaled and added in fp32.  y (m, n) row-major in out_dtype; rows of no type
+ * are left as they are.  `workspace`: gphl_segment_mm_fp8_workspace_bytes. */
+int64_t gphl_segment_mm_fp8_workspace_bytes(int64_t n_types, int32_t typed, int64_t m, int64_t k, int64_t n);
+int gphl_segment_mm_fp8(int64_t n_types, const int32_t *type_pointer, int64_t m, int64_t k, int64_t n, const void *x, int64_t x_stride,
+                        const float *x_scales, int64_t scale_row_stride, int64_t scale_block_stride, const void *w, int64_t w_stride,
+                        const float *w_scales, int32_t out_dtype, void *y, void *workspace, void *stream);
+
+/* Gated feed-forward h = act(x Wg) * (x Wu), both projections, the activation and the product in one kernel.  x (m, k), row stride ldx;
+ * weights (k, f) with row stride ldw, or, `w_transposed`, (f, k) with row stride ldw; h (m, f) contiguous; dtype bf16 or fp16, sums
+ * fp32.  g, u (both or neither): the two projections in fp32, row stride ld_gu (a multiple of 4), for the backward pass. */
+int64_t gphl_gated_workspace_bytes(int64_t m, int64_t k, int64_t f);
+int gphl_gated(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t f, const void *x, int64_t ldx, const void *wg, const void *wu,
+               int64_t ldw, int32_t w_transposed, void *h, float *g, float *u, int64_t ld_gu, void *workspace, void *stream);
+/* Its backward pass: dg = dh u act'(g), du = dh act(g) (rounded to dtype), dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du.
+ * dx (m, k) and dWg, dWu (laid out as the weights, contiguous) may each be NULL when not wanted (the two weights' together). */
+int64_t gphl_gated_grad_workspace_bytes(int64_t m, int64_t k, int64_t f);
+int gphl_gated_grad(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t f, const void *dh, const float *g, const float *u, int64_t ld_gu,
+                    const void *x, int64_t ldx, const void *wg, const void *wu, int64_t ldw, int32_t w_transposed, void *dx, void *dwg,
+                    void *dwu, void *workspace, void *stream);
+/* The same block on codes (weights (1, f, k)): h in out_dtype (m, f) contiguous, or, q not NULL, as codes with row stride q_stride and
+ * scales (h is then not written). */
+int64_t gphl_gated_fp8_workspace_bytes(int64_t m, int64_t k, int64_t f, int32_t codes_out);
+int gphl_gated_fp8(int32_t act, int64_t m, int64_t k, int64_t f, const void *x, int64_t x_stride, const float *x_scales,
+                   int64_t scale_row_stride, int64_t scale_block_stride, const void *wg, const float *wg_scales, const void *wu,
+                   const float *wu_scales, int64_t w_stride, int32_t out_dtype, void *h, void *q, int64_t q_stride, float *scales,
+                   int64_t scale_stride, void *workspace, void *stream);
 
 #ifdef __cplusplus
 }
