@@ -92,21 +92,21 @@ def build_kernels(force: bool = False, verbose: bool = False, ptxas_info: bool =
 
 
 def build_torch_ops(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the TorchScript registration library with g++ against the installed torch."""
+    """Compile the TorchScript registrations with g++ against the installed torch into one library."""
     import torch
     from torch.utils import cpp_extension as ce
 
     LIB.mkdir(exist_ok=True)
     out = LIB / "libgraphiler.so"
-    src = CSRC / "torch_ops.cpp"
-    deps = [src, ROOT / "include" / "gphl.h", LIB / "libgphl.so"]
+    srcs = [CSRC / "torch_ops.cpp", CSRC / "dense_ops.cpp"]
+    deps = [*srcs, ROOT / "include" / "gphl.h", LIB / "libgphl.so"]
     if not force and not _stale(out, deps):
         return out
     inc = [f"-I{p}" for p in ce.include_paths()] + [f"-I{ROOT / 'include'}", "-I/usr/local/cuda/include"]
     torch_lib = Path(torch.__file__).parent / "lib"
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-DNDEBUG", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-           *inc, src, "-o", out,
+           *inc, *srcs, "-o", out,
            f"-L{LIB}", "-lgphl", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-lc10", "-ltorch_cuda", "-lc10_cuda",
            "-L/usr/local/cuda/lib64", "-lcudart",
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}", "-Wl,--no-as-needed"]

@@ -566,11 +566,7 @@ def linear_fanout(x, w, fan: FanOut, row_scale=None, relu: bool = False, out=Non
 
 
 # ---- dense operators of a transformer block on node rows ------------------------------------------------------------
-
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2}
-FP8_BLOCK = 128
-
+# These go through the TorchScript registrations (csrc/dense_ops.cpp) instead of ctypes: a call of few rows is bound by the host.
 
 class Fp8Rows(NamedTuple):
     """Rows in 8 bits: e4m3 ``values`` (m, k), rows starting on 16-byte boundaries, and float32 ``scales`` (m, ceil(k / 128)) of any
@@ -586,286 +582,98 @@ class Fp8Weight(NamedTuple):
     scales: torch.Tensor
 
 
-def _round_up(v: int, to: int) -> int:
-    return -(-v // to) * to
+_OPS = {}
 
 
-def _dtype(t, what: str, among=DTYPES) -> int:
-    if t.dtype not in among:
-        raise GphlError(f"{what} must be " + " or ".join(str(d).replace("torch.", "") for d in among) + f", not {t.dtype}")
-    return DTYPES[t.dtype]
+def _op(name: str):
+    """my_ops::name; loads the registrations unless the process has them (a copy installed where the reference loads it counts)."""
+    fn = _OPS.get(name)
+    if fn is None:
+        if not hasattr(torch.ops.my_ops, name):
+            if not TORCH_OPS_LIB.exists():
+                raise GphlError(f"{TORCH_OPS_LIB} is missing: run `python -m graphiler_b200.build` (there is no fallback path)")
+            torch.ops.load_library(str(TORCH_OPS_LIB))
+        fn = _OPS[name] = getattr(torch.ops.my_ops, name).default
+    return fn
 
 
-def _workspace(nbytes: int, device):
-    """Scratch from the caching allocator (None: none needed): stream-ordered, and private to a graph that captures the call."""
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def _norm_args(x, weight, eps: float, residual, what: str):
-    _dev(x, weight, residual)
-    if x.dim() != 2 or weight.shape != (x.shape[1],):
-        raise GphlError(f"{what} needs rows (m, n) and a weight of n values")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise GphlError(f"{what}: the residual must have the rows' shape and type")
-    dt = _dtype(x, f"{what}: rows")
-    if weight.dtype not in (x.dtype, torch.float32):
-        raise GphlError(f"{what}: the weight must have the rows' type or be float32")
-    if not eps >= 0:
-        raise GphlError(f"{what}: eps must not be negative")
-    return dt, DTYPES[weight.dtype]
+def _call(name: str, *args):
+    try:
+        return (_OPS.get(name) or _op(name))(*args)
+    except RuntimeError as e:
+        if type(e) is RuntimeError:                    # a refusal of the operator; other kinds (out of memory) keep theirs
+            raise GphlError(str(e).split("\n")[0]) from None
+        raise
 
 
 def rms_norm(x, weight, eps: float = 1e-6, residual=None, return_rstd: bool = False):
-    """Root-mean-square norm of rows: ``y = r * weight / sqrt(mean(r^2) + eps)`` with ``r = x``, or, with a ``residual``, ``r = x +
-    residual`` rounded to the rows' type.  Returns y, (y, r) with a residual; with ``return_rstd`` also 1 / sqrt(..) per row
-    (float32), which ``rms_norm_grad`` takes.  No gradients are recorded: see ``graphiler_b200.dense``."""
-    dt, wdt = _norm_args(x, weight, eps, residual, "rms_norm")
-    y = torch.empty_like(x)
-    r = torch.empty_like(x) if residual is not None else None
-    rstd = torch.empty(x.shape[0], dtype=torch.float32, device=x.device) if return_rstd else None
-    with torch.cuda.device(x.device):
-        _check(lib().gphl_rms_norm(dt, x.shape[0], x.shape[1], _ptr(x), _ptr(residual), _ptr(weight), wdt, eps, _ptr(y), _ptr(r),
-                                   _ptr(rstd), _stream(x)), "rms_norm")
-    out = (y,) + ((r,) if r is not None else ()) + ((rstd,) if return_rstd else ())
-    return out if len(out) > 1 else y
+    """Root-mean-square norm of rows (m, n): ``y = r * weight / sqrt(mean(r^2) + eps)`` with ``r = x``, or, with a ``residual``, ``r = x +
+    residual`` rounded to the rows' type (float32, bfloat16 or float16; the weight has it too or is float32).  Returns y, (y, r) with a
+    residual; with ``return_rstd`` also 1 / sqrt(..) per row (float32), which ``rms_norm_grad`` takes.  No gradients are recorded: see
+    ``graphiler_b200.dense``."""
+    out = _call("rms_norm_rows", x, weight, eps, residual, return_rstd)
+    return tuple(out) if len(out) > 1 else out[0]
 
 
 def rms_norm_grad(r, weight, rstd, dy, dr=None):
     """Gradients of ``rms_norm`` from its r and rstd: (dx, dweight); dx is the residual's gradient too.  ``dr``: the gradient that
     arrives at r itself."""
-    _dev(r, weight, rstd, dy, dr)
-    dt, wdt = _norm_args(r, weight, 0.0, None, "rms_norm_grad")
-    for t in (dy, dr):
-        if t is not None and (t.shape != r.shape or t.dtype != r.dtype):
-            raise GphlError("rms_norm_grad: gradients must have the rows' shape and type")
-    if rstd.dtype != torch.float32 or rstd.shape != (r.shape[0],):
-        raise GphlError("rms_norm_grad: rstd must hold one float32 per row")
-    dx, dw = torch.empty_like(r), torch.empty_like(weight)
-    m, n = r.shape
-    with torch.cuda.device(r.device):
-        ws = _workspace(int(lib().gphl_rms_norm_grad_workspace_bytes(dt, m, n)), r.device)
-        _check(lib().gphl_rms_norm_grad(dt, m, n, _ptr(r), _ptr(weight), wdt, _ptr(rstd), _ptr(dy), _ptr(dr), _ptr(dx), _ptr(dw), _ptr(ws),
-                                        _stream(r)), "rms_norm_grad")
-    return dx, dw
-
-
-def _new_fp8_rows(m: int, n: int, device) -> Fp8Rows:
-    """Empty codes as the quantisers lay them out: rows padded to 16 bytes, a block's scales of consecutive rows together."""
-    q = torch.empty((m, _round_up(n, 16)), dtype=torch.float8_e4m3fn, device=device)
-    return Fp8Rows(q[:, :n], torch.empty((_round_up(n, FP8_BLOCK) // FP8_BLOCK, m), dtype=torch.float32, device=device).t())
+    return _call("rms_norm_grad", r, weight, rstd, dy, dr)
 
 
 def rms_norm_fp8(x, weight, eps: float = 1e-6, residual=None):
     """``rms_norm`` with y in 8 bits (``Fp8Rows``), each code the correct rounding of the normalised value; scales are powers of two.
     Returns y, or (y, r) with a residual."""
-    dt, wdt = _norm_args(x, weight, eps, residual, "rms_norm_fp8")
-    m, n = x.shape
-    y = _new_fp8_rows(m, n, x.device)
-    r = torch.empty_like(x) if residual is not None else None
-    with torch.cuda.device(x.device):
-        _check(lib().gphl_rms_norm_fp8(dt, m, n, _ptr(x), _ptr(residual), _ptr(weight), wdt, eps, _ptr(y.values), _round_up(n, 16),
-                                       _ptr(y.scales), m, _ptr(r), _stream(x)), "rms_norm_fp8")
-    return y if r is None else (y, r)
+    out = _call("rms_norm_fp8", x, weight, eps, residual)
+    y = Fp8Rows(out[0], out[1])
+    return y if residual is None else (y, out[2])
 
 
 def quantize_fp8(x) -> Fp8Rows:
     """Rows (m, k) in 8 bits: per row and block of 128 columns the smallest power of two that brings the block's largest finite
     magnitude to at most 448, codes rounded to nearest even; non-finite values become NaN."""
-    _dev(x)
-    dt = _dtype(x, "quantize_fp8: rows")
-    if x.dim() != 2:
-        raise GphlError("quantize_fp8 needs rows (m, k)")
-    m, n = x.shape
-    y = _new_fp8_rows(m, n, x.device)
-    with torch.cuda.device(x.device):
-        _check(lib().gphl_quantize_fp8(dt, m, n, _ptr(x), _ptr(y.values), _round_up(n, 16), _ptr(y.scales), m, _stream(x)), "quantize_fp8")
-    return y
+    return Fp8Rows(*_call("quantize_fp8", x))
 
 
 def quantize_fp8_weight(w) -> Fp8Weight:
     """Weights (k, n) or (types, k, n), as ``segment_mm`` takes them, in 8 bits with a power-of-two scale per 128 x 128 values."""
-    _dev(w)
-    dt = _dtype(w, "quantize_fp8_weight: weights")
-    if w.dim() not in (2, 3):
-        raise GphlError("quantize_fp8_weight needs (k, n) or (types, k, n)")
-    t, (k, n) = (w.shape[0] if w.dim() == 3 else 1), w.shape[-2:]
-    q = torch.empty((t, n, _round_up(k, 16)), dtype=torch.float8_e4m3fn, device=w.device)
-    s = torch.empty((t, _round_up(n, FP8_BLOCK) // FP8_BLOCK, _round_up(k, FP8_BLOCK) // FP8_BLOCK), dtype=torch.float32, device=w.device)
-    with torch.cuda.device(w.device):
-        _check(lib().gphl_quantize_fp8_weight(dt, t, k, n, _ptr(w), _ptr(q), _round_up(k, 16), _ptr(s), _stream(w)), "quantize_fp8_weight")
-    return Fp8Weight(q[:, :, :k], s)
-
-
-def _codes(values, scales, ndim: int, what: str):
-    """Checks a pair of codes and scales; returns the row stride in bytes."""
-    if not values.is_cuda or not scales.is_cuda:
-        raise GphlError("operators need CUDA tensors (there is no CPU path)")
-    if values.device != scales.device:
-        raise GphlError("all tensors must live on one device")
-    if values.dtype != torch.float8_e4m3fn or scales.dtype != torch.float32 or values.dim() != ndim or scales.dim() != ndim:
-        raise GphlError(f"{what} must be float8_e4m3fn values with float32 scales, both of {ndim} dimensions")
-    k, n = values.shape[-1], values.shape[-2]
-    blocks = lambda v: _round_up(v, FP8_BLOCK) // FP8_BLOCK
-    want = (n, blocks(k)) if ndim == 2 else (values.shape[0], blocks(n), blocks(k))
-    if scales.shape != want:
-        raise GphlError(f"{what}: scales of shape {tuple(scales.shape)}, {want} are needed")
-    if values.numel() == 0:
-        return _round_up(max(k, 1), 16)
-    # strides of dimensions of one element say nothing
-    row = values.stride(-2) if n > 1 else (values.stride(0) // n if ndim == 3 and values.shape[0] > 1 else _round_up(k, 16))
-    whole = ndim == 2 or values.shape[0] == 1 or values.stride(0) == n * row
-    if (k > 1 and values.stride(-1) != 1) or row % 16 or row < k or not whole or values.data_ptr() % 16:
-        raise GphlError(f"{what}: rows of codes must be contiguous and start on 16-byte boundaries, equally far apart (as the quantisers lay them out)")
-    if ndim == 3 and not scales.is_contiguous():
-        raise GphlError(f"{what}: scales must be contiguous")
-    return row
+    return Fp8Weight(*_call("quantize_fp8_weight", w))
 
 
 def dequantize_fp8(q: Fp8Rows, dtype=torch.float32):
     """The values that rows in 8 bits stand for.  bfloat16 holds them exactly when the scales are powers of two."""
-    row = _codes(q.values, q.scales, 2, "dequantize_fp8: rows")
-    if dtype not in DTYPES:
-        raise GphlError("dequantize_fp8: float32, bfloat16 or float16")
-    m, n = q.values.shape
-    y = torch.empty((m, n), dtype=dtype, device=q.values.device)
-    with torch.cuda.device(y.device):
-        _check(lib().gphl_dequantize_fp8(DTYPES[dtype], m, n, _ptr(q.values), row, _ptr(q.scales), q.scales.stride(0), q.scales.stride(1),
-                                         _ptr(y), _stream(y)), "dequantize_fp8")
-    return y
+    return _call("dequantize_fp8", q.values, q.scales, dtype)
 
 
 def segment_mm_fp8(x: Fp8Rows, w: Fp8Weight, type_pointer=None, out_dtype=torch.bfloat16, out=None):
     """``segment_mm`` on rows and weights in 8 bits: y[p_t:p_{t+1}] = x[p_t:p_{t+1}] @ w[t], blocks of 128 scaled and summed in float32.
     ``type_pointer`` (types + 1) int32, or None with one type for all rows.  Rows that no type covers are left as they are (of a
     new ``out``: undefined)."""
-    xrow, wrow = _codes(x.values, x.scales, 2, "segment_mm_fp8: rows"), _codes(w.values, w.scales, 3, "segment_mm_fp8: weights")
-    (m, k), (t, n, wk) = x.values.shape, w.values.shape
-    if wk != k:
-        raise GphlError("inner dimensions differ")
-    dev = x.values.device
-    if _dev(type_pointer, out) not in (None, dev) or w.values.device != dev:
-        raise GphlError("all tensors must live on one device")
-    if type_pointer is None and t != 1:
-        raise GphlError("segment_mm_fp8: several types need a type pointer")
-    if type_pointer is not None and (type_pointer.dtype != torch.int32 or type_pointer.numel() != t + 1):
-        raise GphlError("segment_mm_fp8: the type pointer must hold types + 1 int32 values")
-    if out is not None:
-        if out.shape != (m, n):
-            raise GphlError("segment_mm_fp8: out must be (m, n)")
-        out_dtype = out.dtype
-    if out_dtype not in DTYPES:
-        raise GphlError("segment_mm_fp8: float32, bfloat16 or float16 output")
-    y = out if out is not None else torch.empty((m, n), dtype=out_dtype, device=dev)
-    if k == 0:
-        return y.zero_()
-    with torch.cuda.device(dev):
-        ws = _workspace(int(lib().gphl_segment_mm_fp8_workspace_bytes(t, type_pointer is not None, m, k, n)), dev)
-        _check(lib().gphl_segment_mm_fp8(t, _ptr(type_pointer), m, k, n, _ptr(x.values), xrow, _ptr(x.scales), x.scales.stride(0),
-                                         x.scales.stride(1), _ptr(w.values), wrow, _ptr(w.scales), DTYPES[out_dtype], _ptr(y), _ptr(ws),
-                                         _stream(y)), "segment_mm_fp8")
-    return y
-
-
-def _rows16(t):
-    """(tensor, row stride) of a contiguous 16-bit matrix in rows that start on 16-byte boundaries: the tensor itself, or a padded copy."""
-    m, n = t.shape
-    if n % 8 == 0 and t.data_ptr() % 16 == 0:
-        return t, n
-    p = torch.empty((m, _round_up(n, 8)), dtype=t.dtype, device=t.device)
-    _check(lib().gphl_pad_rows_16(m, n, _ptr(t), _ptr(p), _stream(t)), "pad_rows")
-    return p, p.shape[1]
-
-
-def _gated_args(x, w_gate, w_up, activation, what: str):
-    """Checks; returns (dtype, activation, m, k, f, transposed)."""
-    if activation not in ACTIVATIONS:
-        raise GphlError(f"{what}: unknown activation {activation!r} (" + ", ".join(ACTIVATIONS) + ")")
-    if x.dim() != 2 or w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[0] != x.shape[1]:
-        raise GphlError(f"{what} needs rows (m, k) and two weights (k, f)")
-    dt = _dtype(x, f"{what}: rows", (torch.bfloat16, torch.float16))
-    if w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
-        raise GphlError(f"{what}: rows and weights must have one type")
-    transposed = not (w_gate.is_contiguous() and w_up.is_contiguous())
-    _dev(x, w_gate.t() if transposed else w_gate, w_up.t() if transposed else w_up)
-    return dt, ACTIVATIONS[activation], x.shape[0], x.shape[1], w_gate.shape[1], transposed
+    return _call("segment_mm_fp8", x.values, x.scales, w.values, w.scales, type_pointer, out_dtype, out)
 
 
 def gated_linear(x, w_gate, w_up, activation: str = "silu", return_projections: bool = False):
-    """Gated feed-forward ``act(x @ w_gate) * (x @ w_up)`` in one kernel.  bfloat16 or float16 rows (m, k) and weights (k, f), each
-    contiguous, or both weights transposed views of contiguous (f, k) tensors; sums in float32.  With ``return_projections``: (h, g, u), the
-    two products in float32 for ``gated_linear_grad``.  No gradients are recorded: see ``graphiler_b200.dense``."""
-    dt, act, m, k, f, tr = _gated_args(x, w_gate, w_up, activation, "gated_linear")
-    dev = x.device
-    h = torch.empty((m, f), dtype=x.dtype, device=dev)
-    g = u = None
-    ld = _round_up(f, 4)
-    if return_projections:
-        g, u = (torch.empty((m, ld), dtype=torch.float32, device=dev) for _ in range(2))
-    if k == 0:
-        h.zero_()
-        return (h, g.zero_(), u.zero_()) if return_projections else h
-    with torch.cuda.device(dev):
-        xs, ldx = _rows16(x)
-        (wg, ldw), (wu, _) = (_rows16(w.t() if tr else w) for w in (w_gate, w_up))
-        ws = _workspace(int(lib().gphl_gated_workspace_bytes(m, k, f)), dev)
-        _check(lib().gphl_gated(dt, act, m, k, f, _ptr(xs), ldx, _ptr(wg), _ptr(wu), ldw, tr, _ptr(h), _ptr(g), _ptr(u), ld, _ptr(ws),
-                                _stream(x)), "gated_linear")
-    return (h, g, u) if return_projections else h
+    """Gated feed-forward ``act(x @ w_gate) * (x @ w_up)`` in one kernel; ``activation``: silu, gelu (the exact form) or relu.  bfloat16 or
+    float16 rows (m, k) and weights (k, f), each contiguous, or both weights transposed views of contiguous (f, k) tensors; sums in
+    float32.  With ``return_projections``: (h, g, u), the two products in float32 with rows padded to a multiple of 4 columns, for
+    ``gated_linear_grad``.  No gradients are recorded: see ``graphiler_b200.dense``."""
+    out = _call("gated_linear_rows", x, w_gate, w_up, activation, return_projections)
+    return tuple(out) if return_projections else out[0]
 
 
 def gated_linear_grad(dh, g, u, x, w_gate, w_up, activation: str = "silu", want_dx: bool = True, want_dw: bool = True):
-    """Gradients of ``gated_linear`` from its projections: (dx, dw_gate, dw_up), the weights' laid out as the weights; None where
-    not wanted."""
-    dt, act, m, k, f, tr = _gated_args(x, w_gate, w_up, activation, "gated_linear_grad")
-    _dev(x, dh, g, u)
-    if dh.shape != (m, f) or dh.dtype != x.dtype:
-        raise GphlError("gated_linear_grad: dh must have the output's shape and type")
-    ld = _round_up(f, 4)
-    if g.shape != (m, ld) or u.shape != (m, ld) or g.dtype != torch.float32 or u.dtype != torch.float32:
-        raise GphlError("gated_linear_grad: g and u must be the projections that gated_linear returned")
-    dev = x.device
-    dx = torch.empty_like(x) if want_dx else None
-    dwg, dwu = (torch.empty((f, k) if tr else (k, f), dtype=x.dtype, device=dev) if want_dw else None for _ in range(2))
-    with torch.cuda.device(dev):
-        xs, ldx = _rows16(x) if want_dw else (x, k)
-        (wg, ldw), (wu, _) = (_rows16(w.t() if tr else w) if want_dx else (None, k if tr else f) for w in (w_gate, w_up))
-        ws = _workspace(int(lib().gphl_gated_grad_workspace_bytes(m, k, f)), dev)
-        _check(lib().gphl_gated_grad(dt, act, m, k, f, _ptr(dh), _ptr(g), _ptr(u), ld, _ptr(xs), ldx, _ptr(wg), _ptr(wu), ldw, tr, _ptr(dx),
-                                     _ptr(dwg), _ptr(dwu), _ptr(ws), _stream(x)), "gated_linear_grad")
-    return dx, (dwg.t() if tr else dwg) if want_dw else None, (dwu.t() if tr else dwu) if want_dw else None
+    """Gradients of ``gated_linear``: (dx, dw_gate, dw_up), the weights' laid out as the weights; None where not wanted.  ``g``, ``u``: the
+    projections that ``gated_linear`` returned, or None: they are made again."""
+    out = _call("gated_linear_grad", dh, g, u, x, w_gate, w_up, activation, want_dx, want_dw)
+    dx = out[0] if want_dx else None
+    return (dx,) + (tuple(out[-2:]) if want_dw else (None, None))
 
 
 def gated_linear_fp8(x: Fp8Rows, w_gate: Fp8Weight, w_up: Fp8Weight, activation: str = "silu", out_dtype=torch.float8_e4m3fn):
     """``gated_linear`` on rows and weights (one type) in 8 bits.  The result as ``Fp8Rows``, ready for the next product, or as a tensor
     of ``out_dtype`` float32, bfloat16 or float16."""
-    if activation not in ACTIVATIONS:
-        raise GphlError(f"gated_linear_fp8: unknown activation {activation!r} (" + ", ".join(ACTIVATIONS) + ")")
-    xrow = _codes(x.values, x.scales, 2, "gated_linear_fp8: rows")
-    wrow, urow = (_codes(w.values, w.scales, 3, "gated_linear_fp8: weights") for w in (w_gate, w_up))
-    (m, k), (t, f, wk) = x.values.shape, w_gate.values.shape
-    if w_up.values.shape != w_gate.values.shape or t != 1 or wk != k:
-        raise GphlError("gated_linear_fp8 needs two weights (1, f, k) and rows (m, k)")
-    if urow != wrow:
-        raise GphlError("gated_linear_fp8: the two weights must be laid out alike")
-    dev = x.values.device
-    if w_gate.values.device != dev or w_up.values.device != dev:
-        raise GphlError("all tensors must live on one device")
-    codes = out_dtype == torch.float8_e4m3fn
-    if not codes and out_dtype not in DTYPES:
-        raise GphlError("gated_linear_fp8: float8_e4m3fn, float32, bfloat16 or float16 output")
-    if k == 0:
-        z = torch.zeros((m, f), dtype=torch.float32 if codes else out_dtype, device=dev)
-        return quantize_fp8(z) if codes else z
-    q = _new_fp8_rows(m, f, dev) if codes else None
-    h = None if codes else torch.empty((m, f), dtype=out_dtype, device=dev)
-    with torch.cuda.device(dev):
-        ws = _workspace(int(lib().gphl_gated_fp8_workspace_bytes(m, k, f, codes)), dev)
-        _check(lib().gphl_gated_fp8(ACTIVATIONS[activation], m, k, f, _ptr(x.values), xrow, _ptr(x.scales), x.scales.stride(0),
-                                    x.scales.stride(1), _ptr(w_gate.values), _ptr(w_gate.scales), _ptr(w_up.values), _ptr(w_up.scales), wrow,
-                                    0 if codes else DTYPES[out_dtype], _ptr(h), _ptr(q.values) if codes else None, _round_up(f, 16),
-                                    _ptr(q.scales) if codes else None, m, _ptr(ws), c_void_p(torch.cuda.current_stream(dev).cuda_stream)),
-               "gated_linear_fp8")
-    return q if codes else h
+    out = _call("gated_linear_fp8", x.values, x.scales, w_gate.values, w_gate.scales, w_up.values, w_up.scales, activation, out_dtype)
+    return Fp8Rows(*out) if len(out) > 1 else out[0]
 
 
 def tc_wait_timeouts() -> int:

@@ -1,29 +1,16 @@
 // Gated feed-forward h = act(x Wg) * (x Wu) and its backward pass, on the product of tc_gemm.cu.
 //
 // Forward: one launch; a tile multiplies the same rows by columns of both weights, so that g and u of an element meet in one
-// thread.  With gradients wanted, g and u are stored in fp32: recomputing them would cost 4 m k f more operations (a third of the step),
-// and 16-bit copies would add their rounding to dg and du.  Backward: one elementwise pass makes dg and du (16 bits, as any
-// gradient between two products), then dx = [dg du] [Wg Wu]^T as one product over both pairs, and dWg, dWu as one launch of two.
+// thread.  Backward: dg and du (rounded to 16 bits, as any gradient between two products), then dx = [dg du] [Wg Wu]^T as one product
+// over both pairs, and dWg, dWu as one launch of two.  dg and du come from g and u in fp32 (16-bit copies would add their
+// rounding): either stored by the forward pass and read by an elementwise kernel, or made again by the forward's product with dh in its
+// epilogue, which costs 4 m k f operations and saves 16 bytes an element.
 #include <algorithm>
 
 #include "rows.cuh"
 #include "tc_gemm.cuh"
 
 namespace gphl {
-
-__device__ __forceinline__ void gate_grads(float dh, float g, float u, int act, float &dg, float &du) {
-  float h, d;                                          // act(g) and act'(g)
-  if (act == ACT_SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-g));
-    h = g * s, d = s * (1.f + g * (1.f - s));
-  } else if (act == ACT_GELU) {
-    const float c = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-    h = g * c, d = c + g * 0.39894228040143268f * __expf(-0.5f * g * g);
-  } else {
-    h = activate(g, ACT_RELU), d = g > 0.f ? 1.f : 0.f;
-  }
-  dg = dh * u * d, du = dh * h;
-}
 
 // A thread per 8 columns of a row; dg and du have rows of ld (a multiple of 8), g and u of ld_gu (a multiple of 4).
 template <typename T>
@@ -52,12 +39,14 @@ __global__ void __launch_bounds__(256) gate_grads_kernel(const T *__restrict__ d
     uu[j] = y.x, uu[j + 1] = y.y, uu[j + 2] = y.z, uu[j + 3] = y.w;
   }
   uint4 og, ou;
+  with_activation(act, [&](auto k) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) gate_grads<decltype(k)::value>(a[j], gg[j], uu[j]);
+  });
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    float p, q;
-    gate_grads(a[j], gg[j], uu[j], act, p, q);
-    reinterpret_cast<T *>(&og)[j] = from_float<T>(p);
-    reinterpret_cast<T *>(&ou)[j] = from_float<T>(q);
+    reinterpret_cast<T *>(&og)[j] = from_float<T>(gg[j]);
+    reinterpret_cast<T *>(&ou)[j] = from_float<T>(uu[j]);
   }
   *reinterpret_cast<uint4 *>(dg + row * ld + c) = og;
   *reinterpret_cast<uint4 *>(du + row * ld + c) = ou;
@@ -75,6 +64,11 @@ static int gated_sizes(int32_t act, int64_t m, int64_t k, int64_t f) {
 static GemmCall forward_call(int dtype, int act, int64_t m, int64_t k, int64_t f) {
   GemmCall c;
   c.in_type = c.out_type = dtype, c.dual = DUAL_GATED, c.m = m, c.n = f, c.k = k, c.act = act, c.ld_out = f;
+  return c;
+}
+static GemmCall grads_call(int dtype, int act, int64_t m, int64_t k, int64_t f) {
+  GemmCall c = forward_call(dtype, act, m, k, f);
+  c.dual = DUAL_GATED_GRAD, c.ld_out = up(f, 8);
   return c;
 }
 static GemmCall dx_call(int dtype, int64_t m, int64_t k, int64_t f) {
@@ -114,12 +108,12 @@ extern "C" int gphl_gated(int32_t dtype, int32_t act, int64_t m, int64_t k, int6
   return gemm(c, "gated", static_cast<cudaStream_t>(stream_));
 }
 
-// Workspace: dg and du, then the larger of the two products' own.
+// Workspace: dg and du, then the largest of the products' own.
 extern "C" int64_t gphl_gated_grad_workspace_bytes(int64_t m, int64_t k, int64_t f) {
   if (m <= 0 || k <= 0 || f <= 0) return 0;
   const int64_t grads = 2 * up(m * up(f, 8) * 2, 256);
-  return grads + std::max(gemm_workspace_bytes(dx_call(GPHL_BF16, m, k, f)), std::max(gemm_workspace_bytes(dw_call(GPHL_BF16, m, k, f, false)),
-                                                                                     gemm_workspace_bytes(dw_call(GPHL_BF16, m, k, f, true))));
+  return grads + std::max({gemm_workspace_bytes(grads_call(GPHL_BF16, 0, m, k, f)), gemm_workspace_bytes(dx_call(GPHL_BF16, m, k, f)),
+                           gemm_workspace_bytes(dw_call(GPHL_BF16, m, k, f, false)), gemm_workspace_bytes(dw_call(GPHL_BF16, m, k, f, true))});
 }
 
 extern "C" int gphl_gated_grad(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t f, const void *dh, const float *g, const float *u, int64_t ld_gu,
@@ -138,39 +132,45 @@ extern "C" int gphl_gated_grad(int32_t dtype, int32_t act, int64_t m, int64_t k,
     }
     return GPHL_OK;
   }
-  GPHL_REQUIRE(dh && g && u && workspace && (!dx || (wg && wu)) && (!dwg || x), "null pointer argument");
+  GPHL_REQUIRE(dh && !g == !u && workspace && ((!dx && g) || (wg && wu)) && ((!dwg && g) || x), "null pointer argument");
   GPHL_REQUIRE(ldx >= k && ldw >= (w_transposed ? k : f), "gated_grad: rows are shorter than they hold");
-  GPHL_REQUIRE(ld_gu >= f && ld_gu % 4 == 0 && aligned16(g) && aligned16(u), "gated_grad: rows of g and u must start on 16-byte boundaries");
+  GPHL_REQUIRE(!g || (ld_gu >= f && ld_gu % 4 == 0 && aligned16(g) && aligned16(u)), "gated_grad: rows of g and u must start on 16-byte boundaries");
   GPHL_REQUIRE(aligned16(workspace), "gated_grad: the workspace must start on a 16-byte boundary");
   const int64_t ld = up(f, 8), bytes = up(m * ld * 2, 256);
   char *dg = static_cast<char *>(workspace), *du = dg + bytes, *rest = du + bytes;
-  const int64_t threads = m * (ld / 8);
-  GPHL_REQUIRE(threads < (int64_t)INT32_MAX * 256, "size out of range");
-  const bool vec = f % 8 == 0 && aligned16(dh);
-  const unsigned grid = (unsigned)((threads + 255) / 256);
-  if (dtype == GPHL_BF16)
-    gate_grads_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16 *>(dh), g, u, ld_gu, m, f, act, vec,
-                                                               reinterpret_cast<__nv_bfloat16 *>(dg), reinterpret_cast<__nv_bfloat16 *>(du), ld);
-  else
-    gate_grads_kernel<__half><<<grid, 256, 0, stream>>>(static_cast<const __half *>(dh), g, u, ld_gu, m, f, act, vec, reinterpret_cast<__half *>(dg),
-                                                        reinterpret_cast<__half *>(du), ld);
-  rc = launched("gate_grads_kernel");
+  const Matrix rows{x, m, k, ldx};
+  Matrix w[2];
+  for (int i = 0; i < 2; ++i) w[i] = w_transposed ? Matrix{i ? wu : wg, f, k, ldw} : Matrix{i ? wu : wg, k, f, ldw};
+  if (g) {
+    const int64_t threads = m * (ld / 8);
+    GPHL_REQUIRE(threads < (int64_t)INT32_MAX * 256, "size out of range");
+    const bool vec = f % 8 == 0 && aligned16(dh);
+    const unsigned grid = (unsigned)((threads + 255) / 256);
+    if (dtype == GPHL_BF16)
+      gate_grads_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(static_cast<const __nv_bfloat16 *>(dh), g, u, ld_gu, m, f, act, vec,
+                                                                 reinterpret_cast<__nv_bfloat16 *>(dg), reinterpret_cast<__nv_bfloat16 *>(du), ld);
+    else
+      gate_grads_kernel<__half><<<grid, 256, 0, stream>>>(static_cast<const __half *>(dh), g, u, ld_gu, m, f, act, vec, reinterpret_cast<__half *>(dg),
+                                                          reinterpret_cast<__half *>(du), ld);
+    rc = launched("gate_grads_kernel");
+  } else {
+    GemmCall c = grads_call(dtype, act, m, k, f);
+    c.a[0] = rows, c.b[0] = w[0], c.b[1] = w[1], c.b_mn = !w_transposed;
+    c.dh = dh, c.out[0] = dg, c.out[1] = du, c.workspace = rest;
+    rc = gemm(c, "gated_grad", stream);
+  }
   if (rc != GPHL_OK) return rc;
   const Matrix grads[2] = {{dg, m, f, ld}, {du, m, f, ld}};
   if (dx) {
     GemmCall c = dx_call(dtype, m, k, f);
     c.b_mn = w_transposed;
-    for (int i = 0; i < 2; ++i) {
-      c.a[i] = grads[i];
-      c.b[i] = w_transposed ? Matrix{i ? wu : wg, f, k, ldw} : Matrix{i ? wu : wg, k, f, ldw};
-    }
+    for (int i = 0; i < 2; ++i) c.a[i] = grads[i], c.b[i] = w[i];
     c.out[0] = dx, c.workspace = rest;
     rc = gemm(c, "gated_grad", stream);
     if (rc != GPHL_OK) return rc;
   }
   if (dwg) {
     GemmCall c = dw_call(dtype, m, k, f, w_transposed);
-    const Matrix rows{x, m, k, ldx};
     for (int i = 0; i < 2; ++i) c.a[i] = w_transposed ? grads[i] : rows, c.b[i] = w_transposed ? rows : grads[i];
     c.out[0] = dwg, c.out[1] = dwu, c.workspace = rest;
     rc = gemm(c, "gated_grad", stream);

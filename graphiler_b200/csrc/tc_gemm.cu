@@ -1,6 +1,6 @@
 // The tensor-core product of the dense operators for sm_100a: out[i, j] = sum_k A[i, k] B[j, k], 16-bit or e4m3 operands, fp32 sums.
 //
-// One persistent block per SM walks (128 x BN)-tiles of the output.  Ten warps: one brings boxes of A and B into a ring of
+// One persistent block per SM, or one pair of blocks per two SMs, walks tiles of 128 (256) rows x BN columns of the output.  Ten warps: one brings boxes of A and B into a ring of
 // shared-memory stages by TMA (128 bytes of k per stage, 128-byte swizzle), one issues tcgen05.mma into one of two accumulators in
 // TMEM, eight read the other one back and finish the tile, so that loads, products and stores of neighbouring tiles overlap.
 // 16-bit: an accumulator gathers a whole tile.  e4m3: it holds one block of 128 k, which the eight warps scale (row scale x weight
@@ -22,6 +22,8 @@ constexpr int RING_BYTES = 196608;                     // shared memory of the s
 constexpr int STAGING = 4096;                          // per epilogue warp: 32 rows x 128 bytes
 constexpr int GEMM_SMEM = 1024 + RING_BYTES + EPI_WARPS * STAGING;
 constexpr int MAX_STAGES = 8;
+constexpr int SCALES = 16;                             // row scales fetched at a time (blocks of k)
+static_assert(2 * SCALES * 32 * 4 <= STAGING, "two groups of row scales lie in the staging buffer");
 constexpr uint32_t GEMM_WAIT_LIMIT = 1u << 22;
 constexpr int RASTER = 16;                             // row tiles that are walked together across the columns (L2 reuse of both operands)
 
@@ -29,14 +31,16 @@ __device__ int g_gemm_wait_timeouts = 0;
 
 struct __align__(64) GemmArgs {
   CUtensorMap a[2], b[2];
-  int64_t m, n, tiles_m, tiles_n, work;                // work = tiles_m * tiles_n * batch * splits
+  int64_t m, n;
+  uint32_t tiles_m, tiles_n, work;                     // work = tiles_m * tiles_n * batch * splits < 2^31
   int32_t batch, splits, kt, kt_first;                 // steps of 128 bytes of k; kt_first: steps of the first pair (CONCAT)
   int32_t a_mn, b_mn, types, stages;
   uint32_t idesc;
   const int32_t *ptr;
   void *out[2];
   int64_t ld_out;
-  int32_t out_type, out_vec, act;
+  int32_t out_type, out_vec, act, dh_vec;
+  const void *dh;
   float *g, *u;
   int64_t ld_gu;
   uint8_t *q;
@@ -55,8 +59,31 @@ __device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)_
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
 }
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+// The same barrier in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_block(uint32_t bar, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(bar), "r"(rank));
+  return r;
+}
+template <int CTAS> __device__ __forceinline__ void arrive(uint32_t bar) {
+  if constexpr (CTAS == 2) asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+template <int CTAS> __device__ __forceinline__ void alloc(uint32_t to, uint32_t cols) {
+  if constexpr (CTAS == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <int CTAS> __device__ __forceinline__ void dealloc(uint32_t tmem, uint32_t cols) {
+  if constexpr (CTAS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -78,10 +105,19 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   *failed = 1;
   return false;
 }
-__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-               "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-               : "memory");
+// One box into this block's shared memory; its bytes are counted on `bar`, which may lie in the pair's even block.
+template <int CTAS> __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
+  if constexpr (CTAS == 2)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void copy4(float *dst, const float *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
 // Shared-memory operand descriptor, 128-byte swizzle.  K-major: rows of 128 bytes, groups of 8 rows 1024 B apart.  MN-major: rows
 // of 64 i (or j) for one k, groups of 8 k 1024 B apart, the next 64 i 8192 B on (a box is 64 x 64).
@@ -93,18 +129,28 @@ __device__ __forceinline__ uint64_t operand(uint32_t saddr, bool mn) {
   d |= (uint64_t)2 << 61;
   return d;
 }
-template <bool FP8> __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  if constexpr (FP8)
-    asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
-  else
-    asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+#define GPHL_MMA(group, kind)                                                             \
+  asm volatile(                                                                           \
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"                                         \
+      "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n}" ::"r"(d), \
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)                                                \
+      : "memory")
+template <int CTAS, bool FP8> __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if constexpr (CTAS == 2) {
+    if constexpr (FP8) GPHL_MMA("2", "f8f6f4");
+    else GPHL_MMA("2", "f16");
+  } else {
+    if constexpr (FP8) GPHL_MMA("1", "f8f6f4");
+    else GPHL_MMA("1", "f16");
+  }
 }
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+#undef GPHL_MMA
+// Arrives on `bar` (of a pair: of both blocks) once the products issued so far are done.
+template <int CTAS> __device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CTAS == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -141,21 +187,25 @@ struct Tile {
 
 // Work item `w`, found by a whole warp.  Typed: row tile `mt` is looked up in the type pointer, 32 types at a time (tile counts, prefix
 // sum, one hit); pointer values outside [0, m] are clamped.
-__device__ __forceinline__ Tile find_tile(const GemmArgs &a, int64_t w, int bn_out, int lane) {
+template <int CTAS> __device__ __forceinline__ Tile find_tile(const GemmArgs &a, uint32_t w, int bn_out, int lane) {
+  constexpr int TM = GM * CTAS;                          // rows of a tile; t.rows counts those of the whole tile
   Tile t;
-  const int64_t plane = a.tiles_m * a.tiles_n;
-  t.split = (int)(w / (plane * a.batch));
-  w -= t.split * plane * a.batch;
-  t.batch = (int)(w / plane);
-  w -= t.batch * plane;
-  const int64_t band = w / (RASTER * a.tiles_n), in = w - band * RASTER * a.tiles_n;
-  const int64_t high = min((int64_t)RASTER, a.tiles_m - band * RASTER);
-  const int64_t nt = in / high, mt = band * RASTER + (in - nt * high);
+  const uint32_t plane = a.tiles_m * a.tiles_n;
+  t.split = t.batch = 0;
+  if (w >= plane) {
+    const uint32_t p = w / plane;
+    w -= p * plane;
+    t.split = (int)(p / (uint32_t)a.batch), t.batch = (int)(p % (uint32_t)a.batch);
+  }
+  const uint32_t band = w / (RASTER * a.tiles_n), in = w - band * RASTER * a.tiles_n;
+  const uint32_t high = min((uint32_t)RASTER, a.tiles_m - band * RASTER);
+  const uint32_t nt = in / high;
+  const int64_t mt = band * RASTER + (in - nt * high);
   t.n0 = (int)nt * bn_out;
   t.seg = 0;
   if (!a.ptr) {
-    t.row0 = mt * GM;
-    t.rows = (int)min((int64_t)GM, a.m - t.row0);
+    t.row0 = mt * TM;
+    t.rows = (int)min((int64_t)TM, a.m - t.row0);
     return t;
   }
   t.rows = 0, t.row0 = 0;
@@ -167,7 +217,7 @@ __device__ __forceinline__ Tile find_tile(const GemmArgs &a, int64_t w, int bn_o
       lo = min(max((int64_t)__ldg(a.ptr + k), (int64_t)0), a.m);
       hi = min(max((int64_t)__ldg(a.ptr + k + 1), lo), a.m);
     }
-    const int64_t nt_ = (hi - lo + GM - 1) / GM;
+    const int64_t nt_ = (hi - lo + TM - 1) / TM;
     int64_t incl = nt_;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -179,10 +229,10 @@ __device__ __forceinline__ Tile find_tile(const GemmArgs &a, int64_t w, int bn_o
     const unsigned who = __ballot_sync(FULL, hit);
     if (who) {
       const int src = __ffs(who) - 1;
-      const int64_t row = lo + (mt - first) * GM;
+      const int64_t row = lo + (mt - first) * TM;
       t.seg = __shfl_sync(FULL, k, src);
       t.row0 = __shfl_sync(FULL, row, src);
-      t.rows = (int)__shfl_sync(FULL, min((int64_t)GM, hi - row), src);
+      t.rows = (int)__shfl_sync(FULL, min((int64_t)TM, hi - row), src);
       return t;
     }
     base += __shfl_sync(FULL, incl, 31);
@@ -246,6 +296,39 @@ __device__ __forceinline__ void store_chunk(const float (&v)[32], int type, bool
   __syncwarp();
 }
 
+// The reverse for 16-bit rows: 32 columns of the warp's rows, one row per thread; 0 outside.
+__device__ __forceinline__ void load_chunk(float (&v)[32], int type, bool vec, const void *in, int64_t ld, int64_t row0, int rows, int64_t col0, int64_t ncols,
+                                           uint8_t *stg, int lane) {
+  const uint16_t *src = static_cast<const uint16_t *>(in);
+  if (vec && col0 + 32 <= ncols) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = (lane >> 2) + 8 * j, ch = lane & 3;
+      const uint4 p = r < rows ? __ldg(reinterpret_cast<const uint4 *>(src + (row0 + r) * ld + col0 + ch * 8)) : make_uint4(0, 0, 0, 0);
+      *reinterpret_cast<uint4 *>(stg + r * 64 + ((ch ^ ((r >> 1) & 3)) << 4)) = p;
+    }
+  } else {
+    for (int r = 0; r < 32; ++r)
+      *reinterpret_cast<uint16_t *>(stg + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2) =
+          r < rows && col0 + lane < ncols ? __ldg(src + (row0 + r) * ld + col0 + lane) : (uint16_t)0;
+  }
+  __syncwarp();
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint4 p = *reinterpret_cast<const uint4 *>(stg + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4));
+    const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (type == GPHL_BF16) v[8 * q + 2 * j] = __uint_as_float(w[j] << 16), v[8 * q + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      else {
+        const __half2 h = *reinterpret_cast<const __half2 *>(&w[j]);
+        v[8 * q + 2 * j] = __low2float(h), v[8 * q + 2 * j + 1] = __high2float(h);
+      }
+    }
+  }
+  __syncwarp();
+}
+
 // 32 e4m3 codes per row; code rows are padded to 16 bytes, so a 16-byte piece is inside the row whenever its first column is.
 __device__ __forceinline__ void store_code_chunk(const float (&v)[32], float inv, uint8_t *out, int64_t ld, int64_t row0, int rows, int64_t col0,
                                                  int64_t ncols, uint8_t *stg, int lane) {
@@ -273,10 +356,16 @@ __device__ __forceinline__ void store_code_chunk(const float (&v)[32], float inv
 
 // ---- the kernel --------------------------------------------------------------------------------------------------------------------
 
-template <int BN, bool FP8, bool GATED> __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_constant__ GemmArgs a) {
-  constexpr int STAGE = GM * 128 + BN * 128;
+enum Mode { LINEAR, GATED, GATED_GRAD };
+
+// CTAS == 2: a pair of blocks on neighbouring SMs shares a tile of 256 rows: each brings its own 128 rows of A and half of B's columns, the
+// even block issues products over both shared memories (cta_group::2), and every SM reads 64 instead of 96 bytes a cycle for them.
+template <int BN, int CTAS, bool FP8, int MODE> __global__ void __launch_bounds__(GEMM_THREADS, 1) gemm_kernel(const __grid_constant__ GemmArgs a) {
+  constexpr bool PAIRED = MODE != LINEAR;                // two weights, their columns side by side in the accumulator
+  constexpr int BROWS = BN / CTAS;                       // columns of B in this block's shared memory
+  constexpr int STAGE = GM * 128 + BROWS * 128;
   constexpr int STAGES = RING_BYTES / STAGE < MAX_STAGES ? RING_BYTES / STAGE : MAX_STAGES;
-  constexpr int BN_OUT = GATED ? BN / 2 : BN;            // output columns of a tile
+  constexpr int BN_OUT = PAIRED ? BN / 2 : BN;           // output columns of a tile
   constexpr int NCH = BN / 64;                           // chunks of 32 accumulator columns of a thread
   constexpr int KE = FP8 ? 128 : 64;                     // k of a step
   extern __shared__ uint8_t smem_raw[];
@@ -285,6 +374,7 @@ template <int BN, bool FP8, bool GATED> __global__ void __launch_bounds__(GEMM_T
   __shared__ int s_failed;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = CTAS == 2 ? (int)(blockIdx.x & 1) : 0;
   uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const uint32_t ring_u = tc::smem_u32(ring), full = tc::smem_u32(s_full), empty = tc::smem_u32(s_empty);
   const uint32_t acc_full = tc::smem_u32(s_acc_full), acc_empty = tc::smem_u32(s_acc_empty), drain = tc::smem_u32(&s_drain);
@@ -292,58 +382,66 @@ template <int BN, bool FP8, bool GATED> __global__ void __launch_bounds__(GEMM_T
   volatile int *failed = &s_failed;
   uint32_t issued = 0;                                   // TMA warp: steps brought in
 
-  if (warp == EPI_WARPS + 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&s_tmem)), "r"(2 * BN) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  if (warp == EPI_WARPS + 1) tc::alloc<CTAS>(tc::smem_u32(&s_tmem), 2 * BN);
   if (threadIdx.x == 0) {
     s_failed = 0;
     for (int i = 0; i < STAGES; ++i) tc::mbar_init(full + 8 * i, 1), tc::mbar_init(empty + 8 * i, 1);
-    for (int i = 0; i < 2; ++i) tc::mbar_init(acc_full + 8 * i, 1), tc::mbar_init(acc_empty + 8 * i, EPI_WARPS);
+    for (int i = 0; i < 2; ++i) tc::mbar_init(acc_full + 8 * i, 1), tc::mbar_init(acc_empty + 8 * i, CTAS * EPI_WARPS);
     for (int i = 0; i < 4; ++i) tc::mbar_init(pair + 8 * i, 2);
     tc::mbar_init(drain, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   tc::before_sync();
-  __syncthreads();
+  if (CTAS == 2) tc::cluster_sync();                     // the other block's barriers exist before anything arrives there
+  else __syncthreads();
   tc::after_sync();
   const uint32_t tmem = s_tmem;
+  const uint32_t w0 = blockIdx.x / CTAS, wstep = gridDim.x / CTAS;
 
   if (warp == EPI_WARPS) {
-    // ---- TMA: step i goes to stage i % STAGES
+    // ---- TMA: step i goes to stage i % STAGES; the bytes of both blocks are counted on the even block's barrier
     uint32_t i = 0;
     bool ok = true;
-    for (int64_t w = blockIdx.x; w < a.work && ok; w += gridDim.x) {
-      const Tile t = find_tile(a, w, BN_OUT, lane);
+    const uint32_t lead_full = CTAS == 2 ? tc::in_block(full, 0) : full;
+    for (uint32_t w = w0; w < a.work && ok; w += wstep) {
+      const Tile t = find_tile<CTAS>(a, w, BN_OUT, lane);
       if (t.rows == 0) continue;
       const int k0 = (int)((int64_t)a.kt * t.split / a.splits), k1 = (int)((int64_t)a.kt * (t.split + 1) / a.splits);
-      const int brow = t.seg * (int)a.n + t.n0;
+      const int row0 = (int)t.row0 + rank * GM, n0 = t.n0 + (PAIRED ? 0 : rank * BROWS);
+      const int brow = t.seg * (int)a.n + n0;
       if (lane == 0) {
         for (int kt = k0; kt < k1; ++kt, ++i) {
-          const uint32_t s = i % STAGES, bar = full + 8 * s, sa = ring_u + s * STAGE, sb = sa + GM * 128;
+          const uint32_t s = i % STAGES, bar = lead_full + 8 * s, sa = ring_u + s * STAGE, sb = sa + GM * 128;
           if (!(ok = tc::mbar_wait(empty + 8 * s, ((i / STAGES) & 1) ^ 1, failed))) break;
-          tc::mbar_expect_tx(bar, STAGE);
+          if (rank == 0) tc::mbar_expect_tx(full + 8 * s, CTAS * STAGE);
           const int sel = a.batch > 1 ? t.batch : (kt >= a.kt_first), x = (a.batch == 1 && kt >= a.kt_first ? kt - a.kt_first : kt) * KE;
           if (a.a_mn) {
 #pragma unroll
-            for (int c = 0; c < GM / 64; ++c) tc::tma_2d(sa + c * 8192, &a.a[sel], (int)t.row0 + 64 * c, x, bar);
+            for (int c = 0; c < GM / 64; ++c) tc::tma_2d<CTAS>(sa + c * 8192, &a.a[sel], row0 + 64 * c, x, bar);
           } else {
-            tc::tma_2d(sa, &a.a[sel], x, (int)t.row0, bar);
+            tc::tma_2d<CTAS>(sa, &a.a[sel], x, row0, bar);
           }
-          if constexpr (GATED) {
+          if constexpr (PAIRED && CTAS == 2) {           // each block brings one of the two weights
+            if (a.b_mn) {
+#pragma unroll
+              for (int c = 0; c < BROWS / 64; ++c) tc::tma_2d<CTAS>(sb + c * 8192, &a.b[rank], n0 + 64 * c, x, bar);
+            } else {
+              tc::tma_2d<CTAS>(sb, &a.b[rank], x, n0, bar);
+            }
+          } else if constexpr (PAIRED) {
             if (a.b_mn) {
 #pragma unroll
               for (int c = 0; c < BN / 64; ++c)
-                tc::tma_2d(sb + c * 8192, &a.b[c >= BN / 128], t.n0 + 64 * (c % (BN / 128)), x, bar);
+                tc::tma_2d<CTAS>(sb + c * 8192, &a.b[c >= BN / 128], n0 + 64 * (c % (BN / 128)), x, bar);
             } else {
-              tc::tma_2d(sb, &a.b[0], x, t.n0, bar);
-              tc::tma_2d(sb + BN * 64, &a.b[1], x, t.n0, bar);
+              tc::tma_2d<CTAS>(sb, &a.b[0], x, n0, bar);
+              tc::tma_2d<CTAS>(sb + BN * 64, &a.b[1], x, n0, bar);
             }
           } else if (a.b_mn) {
 #pragma unroll
-            for (int c = 0; c < BN / 64; ++c) tc::tma_2d(sb + c * 8192, &a.b[sel], t.n0 + 64 * c, x, bar);
+            for (int c = 0; c < BROWS / 64; ++c) tc::tma_2d<CTAS>(sb + c * 8192, &a.b[sel], n0 + 64 * c, x, bar);
           } else {
-            tc::tma_2d(sb, &a.b[sel], x, brow, bar);
+            tc::tma_2d<CTAS>(sb, &a.b[sel], x, brow, bar);
           }
         }
       }
@@ -351,13 +449,17 @@ template <int BN, bool FP8, bool GATED> __global__ void __launch_bounds__(GEMM_T
       i = __shfl_sync(FULL, i, 0);
     }
     issued = i;
+    // the last steps' stages are given back: after this no commit of the tensor core is on its way to this block's barriers
+    if (lane == 0 && ok)
+      for (uint32_t j = i > STAGES ? i - STAGES : 0; j < i; ++j) tc::mbar_wait(empty + 8 * (j % STAGES), (j / STAGES) & 1, failed);
+    __syncwarp();
   } else if (warp == EPI_WARPS + 1) {
-    // ---- tensor core
+    // ---- tensor core (of a pair: the even block's)
     uint32_t i = 0, acc = 0;                             // acc: accumulators begun (tiles, or blocks of k)
     bool ok = true;
     const uint32_t adv_a = a.a_mn ? 2048 >> 4 : 32 >> 4, adv_b = a.b_mn ? 2048 >> 4 : 32 >> 4;   // one mma's k within a stage
-    for (int64_t w = blockIdx.x; w < a.work && ok; w += gridDim.x) {
-      const Tile t = find_tile(a, w, BN_OUT, lane);
+    for (uint32_t w = w0; w < a.work && ok && rank == 0; w += wstep) {
+      const Tile t = find_tile<CTAS>(a, w, BN_OUT, lane);
       if (t.rows == 0) continue;
       const int k0 = (int)((int64_t)a.kt * t.split / a.splits), k1 = (int)((int64_t)a.kt * (t.split + 1) / a.splits);
       if (lane == 0) {
@@ -370,10 +472,10 @@ template <int BN, bool FP8, bool GATED> __global__ void __launch_bounds__(GEMM_T
           tc::after_sync();
           const uint64_t da = tc::operand(ring_u + s * STAGE, a.a_mn), db = tc::operand(ring_u + s * STAGE + GM * 128, a.b_mn);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) tc::mma<FP8>(d, da + kk * adv_a, db + kk * adv_b, a.idesc, (kk > 0 || (!FP8 && kt > k0)) ? 1u : 0u);
-          tc::commit(empty + 8 * s);
+          for (int kk = 0; kk < 4; ++kk) tc::mma<CTAS, FP8>(d, da + kk * adv_a, db + kk * adv_b, a.idesc, (kk > 0 || (!FP8 && kt > k0)) ? 1u : 0u);
+          tc::commit<CTAS>(empty + 8 * s);
           if (FP8 || kt == k1 - 1) {
-            tc::commit(acc_full + 8 * (acc & 1));
+            tc::commit<CTAS>(acc_full + 8 * (acc & 1));
             ++acc;
           }
         }
@@ -384,58 +486,92 @@ template <int BN, bool FP8, bool GATED> __global__ void __launch_bounds__(GEMM_T
     // ---- epilogue: warp w reads lanes 32 (w % 4) ..; warps 0-3 the first half of the columns, 4-7 the second
     const int half = warp >> 2, quad = warp & 3;
     uint8_t *stg = ring + RING_BYTES + warp * STAGING;
+    const uint32_t lead_empty = CTAS == 2 ? tc::in_block(acc_empty, 0) : acc_empty;
     uint32_t acc = 0, tiles = 0;                         // accumulators read; tiles of codes finished
     bool ok = true;
-    for (int64_t w = blockIdx.x; w < a.work && ok; w += gridDim.x) {
-      const Tile t = find_tile(a, w, BN_OUT, lane);
+    for (uint32_t w = w0; w < a.work && ok; w += wstep) {
+      const Tile t = find_tile<CTAS>(a, w, BN_OUT, lane);
       if (t.rows == 0) continue;
       const int k0 = (int)((int64_t)a.kt * t.split / a.splits), k1 = (int)((int64_t)a.kt * (t.split + 1) / a.splits);
-      const int rows = min(32, t.rows - quad * 32);      // of this warp; may be <= 0
-      const int64_t row0 = t.row0 + quad * 32;
+      const int rows = min(32, t.rows - rank * GM - quad * 32);     // of this warp; may be <= 0
+      const int64_t row0 = t.row0 + rank * GM + quad * 32;
       // accumulator column of chunk c, and the output column that it stands for
-      auto acc_col = [&](int c) { return GATED ? (c < NCH / 2 ? 0 : BN / 2) + half * (BN / 4) + 32 * (c % (NCH / 2 ? NCH / 2 : 1)) : half * (BN / 2) + 32 * c; };
-      auto out_col = [&](int c) { return (int64_t)t.n0 + (GATED ? half * (BN / 4) : half * (BN / 2)) + 32 * c; };
+      auto acc_col = [&](int c) { return PAIRED ? (c < NCH / 2 ? 0 : BN / 2) + half * (BN / 4) + 32 * (c % (NCH / 2 ? NCH / 2 : 1)) : half * (BN / 2) + 32 * c; };
+      auto out_col = [&](int c) { return (int64_t)t.n0 + (PAIRED ? half * (BN / 4) : half * (BN / 2)) + 32 * c; };
       float *part = a.splits > 1 ? a.part + ((int64_t)(t.split * a.batch + t.batch) * a.m) * a.ld_part : nullptr;
+      auto release = [&] {
+        tc::before_sync();
+        __syncwarp();
+        if (lane == 0) tc::arrive<CTAS>(lead_empty + 8 * (acc & 1));
+      };
 
       // one finished chunk of a plain product
       auto put = [&](float (&v)[32], int c) {
         if (part) store_chunk(v, GPHL_F32, true, part, a.ld_part, row0, rows, out_col(c), a.n, stg, lane);
         else store_chunk(v, a.out_type, a.out_vec, a.out[t.batch], a.ld_out, row0, rows, out_col(c), a.n, stg, lane);
       };
-      // one finished pair of chunks of a gated product (g is overwritten by the result)
-      auto put_gated = [&](float (&g)[32], float (&u)[32], int c) {
+      // one finished pair of chunks (g is overwritten by the result)
+      auto put_pair = [&](float (&g)[32], float (&u)[32], int c) {
         if (part) {
           store_chunk(g, GPHL_F32, true, part, a.ld_part, row0, rows, out_col(c), a.n, stg, lane);
           store_chunk(u, GPHL_F32, true, part + a.part_u, a.ld_part, row0, rows, out_col(c), a.n, stg, lane);
+          return;
+        }
+        if constexpr (MODE == GATED_GRAD) {
+          float dh[32];
+          load_chunk(dh, a.out_type, a.dh_vec, a.dh, a.n, row0, rows, out_col(c), a.n, stg, lane);
+          with_activation(a.act, [&](auto k) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) gate_grads<decltype(k)::value>(dh[i], g[i], u[i]);
+          });
+          store_chunk(g, a.out_type, true, a.out[0], a.ld_out, row0, rows, out_col(c), a.ld_out, stg, lane);
+          store_chunk(u, a.out_type, true, a.out[1], a.ld_out, row0, rows, out_col(c), a.ld_out, stg, lane);
           return;
         }
         if (a.g) {
           store_chunk(g, GPHL_F32, true, a.g, a.ld_gu, row0, rows, out_col(c), a.n, stg, lane);
           store_chunk(u, GPHL_F32, true, a.u, a.ld_gu, row0, rows, out_col(c), a.n, stg, lane);
         }
+        with_activation(a.act, [&](auto k) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) g[i] = activate(g[i], a.act) * u[i];
+          for (int i = 0; i < 32; ++i) g[i] = activate<decltype(k)::value>(g[i]) * u[i];
+        });
         if (!FP8 || !a.q) store_chunk(g, a.out_type, a.out_vec, a.out[0], a.ld_out, row0, rows, out_col(c), a.n, stg, lane);
       };
 
       if constexpr (FP8) {
-        float sum[NCH][32];
+        uint64_t sum[NCH][16];                           // pairs of neighbouring columns: packed multiply-adds
 #pragma unroll
         for (int c = 0; c < NCH; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) sum[c][i] = 0.f;
-        const float *sx = a.a_scale + (row0 + min(lane, max(rows, 1) - 1)) * a.a_scale_row;
-        if (rows <= 0) sx = a.a_scale;                   // a row that is stored nowhere
+          for (int i = 0; i < 16; ++i) sum[c][i] = 0;
+        // The row scales of SCALES blocks ahead come into the warp's staging buffer by asynchronous 4-byte copies, two groups in turn (a
+        // load per block into a register left its latency between any two accumulators: 0.72 us a block of a 128 x 256 tile).
+        // Rows that are stored nowhere read the scale of one that is.
+        const float *sx = a.a_scale + (rows > 0 ? row0 + min(lane, rows - 1) : 0) * a.a_scale_row;
+        float *const held = reinterpret_cast<float *>(stg) + lane;                        // block kt at ((kt - k0) % (2 SCALES)) * 32
+        auto fetch = [&](int first) {
+          for (int kt = first; kt < min(first + SCALES, k1); ++kt) tc::copy4(held + ((kt - k0) % (2 * SCALES)) * 32, sx + kt * a.a_scale_block);
+          asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        fetch(k0);
+        fetch(k0 + SCALES);
         // chunk columns of one half lie inside one 128-block of the weight's scales
-        const int nb = min((t.n0 + (GATED ? 0 : half * (BN / 2))) / 128, a.scale_nb - 1);
+        const int nb = min((t.n0 + (PAIRED ? 0 : half * (BN / 2))) / 128, a.scale_nb - 1);
         const float *sw0 = a.b_scale[0] + ((int64_t)t.seg * a.scale_nb + nb) * a.scale_kb;
-        const float *sw1 = GATED ? a.b_scale[1] + (int64_t)nb * a.scale_kb : sw0;
-        float next_x = __ldg(sx + k0 * a.a_scale_block), next_w0 = __ldg(sw0 + k0), next_w1 = GATED ? __ldg(sw1 + k0) : 0.f;
+        const float *sw1 = PAIRED ? a.b_scale[1] + (int64_t)nb * a.scale_kb : sw0;
+        float next_w0 = __ldg(sw0 + k0), next_w1 = PAIRED ? __ldg(sw1 + k0) : 0.f;
         for (int kt = k0; kt < k1; ++kt, ++acc) {
-          const float s0 = next_x * next_w0, s1 = GATED ? next_x * next_w1 : s0;
+          if ((kt - k0) % SCALES == 0) {
+            if (kt > k0) fetch(kt + SCALES);             // into the group that has just been used up (by this thread alone)
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+          }
+          const float x = held[((kt - k0) % (2 * SCALES)) * 32];
+          const float s0 = x * next_w0, s1 = PAIRED ? x * next_w1 : s0;
+          const uint64_t p0 = pack2(s0, s0), p1 = PAIRED ? pack2(s1, s1) : p0;
           if (kt + 1 < k1) {
-            next_x = __ldg(sx + (kt + 1) * a.a_scale_block), next_w0 = __ldg(sw0 + kt + 1);
-            if (GATED) next_w1 = __ldg(sw1 + kt + 1);
+            next_w0 = __ldg(sw0 + kt + 1);
+            if (PAIRED) next_w1 = __ldg(sw1 + kt + 1);
           }
           ok = __all_sync(FULL, tc::mbar_wait(acc_full + 8 * (acc & 1), (acc >> 1) & 1, failed));
           if (!ok) break;
@@ -446,30 +582,40 @@ template <int BN, bool FP8, bool GATED> __global__ void __launch_bounds__(GEMM_T
             float v[32];
             tc::ld32(taddr + acc_col(c), v);
             tc::ld_wait(v);
-            const float s = GATED && c >= NCH / 2 ? s1 : s0;
+            if (c == NCH - 1) release();
+            const uint64_t s = PAIRED && c >= NCH / 2 ? p1 : p0;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) sum[c][i] = fmaf(v[i], s, sum[c][i]);
+            for (int i = 0; i < 16; ++i) sum[c][i] = ffma2(pack2(v[2 * i], v[2 * i + 1]), s, sum[c][i]);
           }
-          tc::before_sync();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(acc_empty + 8 * (acc & 1));
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         if (!ok) break;
-        if constexpr (GATED) {
+        __syncwarp();                                    // the staging buffer changes hands
+        auto unpack = [](const uint64_t (&p)[16], float (&v)[32]) {
 #pragma unroll
-          for (int c = 0; c < NCH / 2; ++c) put_gated(sum[c], sum[c + NCH / 2], c);
+          for (int i = 0; i < 16; ++i) unpack2(p[i], v[2 * i], v[2 * i + 1]);
+        };
+        if constexpr (PAIRED) {
+          float g[NCH / 2][32];
+#pragma unroll
+          for (int c = 0; c < NCH / 2; ++c) {
+            float u[32];
+            unpack(sum[c], g[c]);
+            unpack(sum[c + NCH / 2], u);
+            put_pair(g[c], u, c);
+          }
           if (a.q && !part) {
             // the tile's columns are one block of 128 of the codes, half of it in the warp four further on
             float big = 0.f;
 #pragma unroll
             for (int c = 0; c < NCH / 2; ++c)
 #pragma unroll
-              for (int i = 0; i < 32; ++i) big = fmaxf(big, out_col(c) + i < a.n ? finite_abs(sum[c][i]) : 0.f);
+              for (int i = 0; i < 32; ++i) big = fmaxf(big, out_col(c) + i < a.n ? finite_abs(g[c][i]) : 0.f);
             // (two slots in turn: a slot is written again only after the partner's next arrival, which follows its read)
             const uint32_t slot = 2048 + (tiles & 1) * 128;
             reinterpret_cast<float *>(stg + slot)[lane] = big;
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(pair + 8 * quad);
+            if (lane == 0) tc::arrive<1>(pair + 8 * quad);
             ok = __all_sync(FULL, tc::mbar_wait(pair + 8 * quad, tiles & 1, failed));
             if (!ok) break;
             ++tiles;
@@ -477,23 +623,22 @@ template <int BN, bool FP8, bool GATED> __global__ void __launch_bounds__(GEMM_T
             const int e = fp8_exponent(big);
             if (half == 0 && lane < rows) a.q_scale[(int64_t)(t.n0 / 128) * a.q_scale_stride + row0 + lane] = pow2f(e);
 #pragma unroll
-            for (int c = 0; c < NCH / 2; ++c) store_code_chunk(sum[c], pow2f(-e), a.q, a.ld_out, row0, rows, out_col(c), a.n, stg, lane);
+            for (int c = 0; c < NCH / 2; ++c) store_code_chunk(g[c], pow2f(-e), a.q, a.ld_out, row0, rows, out_col(c), a.n, stg, lane);
           }
         } else {
 #pragma unroll
-          for (int c = 0; c < NCH; ++c) put(sum[c], c);
+          for (int c = 0; c < NCH; ++c) {
+            float v[32];
+            unpack(sum[c], v);
+            put(v, c);
+          }
         }
       } else {
         ok = __all_sync(FULL, tc::mbar_wait(acc_full + 8 * (acc & 1), (acc >> 1) & 1, failed));
         if (!ok) break;
         tc::after_sync();
         const uint32_t taddr = tmem + (acc & 1) * BN + ((uint32_t)(quad * 32) << 16);
-        auto release = [&] {
-          tc::before_sync();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(acc_empty + 8 * (acc & 1));
-        };
-        if constexpr (GATED) {
+        if constexpr (PAIRED) {
 #pragma unroll
           for (int c = 0; c < NCH / 2; ++c) {
             float g[32], u[32];
@@ -502,7 +647,7 @@ template <int BN, bool FP8, bool GATED> __global__ void __launch_bounds__(GEMM_T
             tc::ld_wait(g);
             tc::ld_wait(u);
             if (c == NCH / 2 - 1) release();
-            put_gated(g, u, c);
+            put_pair(g, u, c);
           }
         } else {
 #pragma unroll
@@ -524,22 +669,23 @@ template <int BN, bool FP8, bool GATED> __global__ void __launch_bounds__(GEMM_T
   if (s_failed) {                                        // what is in flight lands before the block leaves
     int unused = 0;
     if (threadIdx.x == 0) atomicAdd(&g_gemm_wait_timeouts, 1);
-    if (warp == EPI_WARPS && lane == 0)
+    if (rank == 0 && warp == EPI_WARPS && lane == 0)     // (the bytes of both blocks are counted on the even block's barriers)
       for (uint32_t j = issued > STAGES ? issued - STAGES : 0; j < issued; ++j) tc::mbar_wait(full + 8 * (j % STAGES), (j / STAGES) & 1, &unused);
-    if (warp == EPI_WARPS + 1 && lane == 0) {
-      tc::commit(drain);
+    if (rank == 0 && warp == EPI_WARPS + 1 && lane == 0) {
+      tc::commit<CTAS>(drain);
       tc::mbar_wait(drain, 0, &unused);
     }
-    __syncthreads();
+    __syncwarp();
   }
-  if (warp == EPI_WARPS + 1)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN) : "memory");
+  if (CTAS == 2) tc::cluster_sync();                     // neither block leaves while the other may reach into its shared memory
+  else __syncthreads();
+  if (warp == EPI_WARPS + 1) tc::dealloc<CTAS>(tmem, 2 * BN);
 }
 
 // ---- joining the parts of a split k ------------------------------------------------------------------------------------------------
 
 // A warp per (row, 128 columns), 4 neighbouring columns a lane; the parts are added in order.
-template <bool GATED> __global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs a) {
+template <int MODE> __global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t blocks = (a.n + 127) / 128, item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
   const int64_t row_b = item / blocks, c0 = (item - row_b * blocks) * 128 + lane * 4;
@@ -553,22 +699,49 @@ template <bool GATED> __global__ void __launch_bounds__(256) gemm_join_kernel(co
       const float *p = a.part + ((int64_t)(s * a.batch + b) * a.m + row) * a.ld_part + c0;
       const float4 v = *reinterpret_cast<const float4 *>(p);
       g.x += v.x, g.y += v.y, g.z += v.z, g.w += v.w;
-      if (GATED) {
+      if (MODE != LINEAR) {
         const float4 t = *reinterpret_cast<const float4 *>(p + a.part_u);
         u.x += t.x, u.y += t.y, u.z += t.z, u.w += t.w;
       }
     }
   }
   float o[4] = {g.x, g.y, g.z, g.w};
-  if (GATED) {
+  if (MODE == GATED_GRAD) {
+    float gg[4] = {g.x, g.y, g.z, g.w}, uu[4] = {u.x, u.y, u.z, u.w}, dh[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t i = row * a.n + c0 + j;
+      dh[j] = c0 + j >= a.n ? 0.f : a.out_type == GPHL_BF16 ? __bfloat162float(static_cast<const __nv_bfloat16 *>(a.dh)[i]) : __half2float(static_cast<const __half *>(a.dh)[i]);
+    }
+    with_activation(a.act, [&](auto k) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) gate_grads<decltype(k)::value>(dh[j], gg[j], uu[j]);
+    });
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c0 + j < a.n) {
+        const int64_t i = row * a.ld_out + c0 + j;
+        if (a.out_type == GPHL_BF16) {
+          static_cast<__nv_bfloat16 *>(a.out[0])[i] = __float2bfloat16_rn(gg[j]);
+          static_cast<__nv_bfloat16 *>(a.out[1])[i] = __float2bfloat16_rn(uu[j]);
+        } else {
+          static_cast<__half *>(a.out[0])[i] = __float2half_rn(gg[j]);
+          static_cast<__half *>(a.out[1])[i] = __float2half_rn(uu[j]);
+        }
+      }
+    return;
+  }
+  if (MODE == GATED) {
     const float gg[4] = {g.x, g.y, g.z, g.w}, uu[4] = {u.x, u.y, u.z, u.w};
     if (a.g && c0 < a.n) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (c0 + j < a.n) a.g[row * a.ld_gu + c0 + j] = gg[j], a.u[row * a.ld_gu + c0 + j] = uu[j];
     }
+    with_activation(a.act, [&](auto k) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = activate(gg[j], a.act) * uu[j];
+      for (int j = 0; j < 4; ++j) o[j] = activate<decltype(k)::value>(gg[j]) * uu[j];
+    });
     if (a.q) {
       float big = 0.f;
 #pragma unroll
@@ -625,12 +798,13 @@ static int encode(CUtensorMap *map, const Matrix &x, int type, bool fp8, int box
 }
 
 struct Shape {
-  int bn, splits;
+  int bn, ctas, splits;
   int64_t tiles_m, tiles_n;
   int32_t kt, batch;
 };
 // The widest tile that leaves no half of it empty (narrower tiles read A once more per column tile) and, parts of 8 steps counted,
 // still gives every SM something; then k split so that the work items fill the SMs: as many parts as make ceil(items / SMs) / items smallest, each of at least 4 steps, fewest parts first.
+static bool paired(const GemmCall &c) { return c.dual == DUAL_GATED || c.dual == DUAL_GATED_GRAD; }
 static Shape shape_of(const GemmCall &c) {
   Shape s{};
   const int ke = c.fp8 ? 128 : 64;
@@ -640,26 +814,29 @@ static Shape shape_of(const GemmCall &c) {
   const int64_t per = (c.k + ke - 1) / ke;
   s.kt = (int32_t)(c.dual == DUAL_CONCAT ? 2 * per : per);
   s.tiles_m = (c.m + GM - 1) / GM + (c.ptr ? std::min<int64_t>(c.types, c.m) : 0);
-  const int64_t wide = c.dual == DUAL_GATED ? 2 * c.n : c.n;
-  s.bn = wide > 128 ? 256 : (wide > 64 || c.dual == DUAL_GATED) ? 128 : 64;
+  const int64_t wide = paired(c) ? 2 * c.n : c.n;
+  s.bn = wide > 128 ? 256 : (wide > 64 || paired(c)) ? 128 : 64;
   if (c.q) s.bn = 256;                                   // a tile is one block of 128 codes
   auto tiles = [&](int bn) { return s.tiles_m * ((wide + bn - 1) / bn) * s.batch; };
   if (s.bn == 256 && !c.q && tiles(256) * std::max(1, s.kt / 8) < sms) s.bn = 128;
-  const int out = c.dual == DUAL_GATED ? s.bn / 2 : s.bn;
+  // pairs of blocks where the tiles of 256 rows are whole but for the last
+  s.ctas = s.bn == 256 && c.m > GM && (!c.ptr || c.m >= 4 * GM * c.types) ? 2 : 1;
+  if (s.ctas == 2) s.tiles_m = (c.m + 2 * GM - 1) / (2 * GM) + (c.ptr ? std::min<int64_t>(c.types, c.m) : 0);
+  const int out = paired(c) ? s.bn / 2 : s.bn, units = sms / s.ctas;
   s.tiles_n = (c.n + out - 1) / out;
   s.splits = 1;
   const int64_t items = s.tiles_m * s.tiles_n * s.batch;
-  if (items < 2 * sms) {
+  if (items < 2 * units) {
     double best = 1e30;
     for (int p = 1; p <= 64 && p * 4 <= s.kt; ++p) {
-      const double waves = (double)((items * p + sms - 1) / sms) / p;      // time in units of one unsplit tile
+      const double waves = (double)((items * p + units - 1) / units) / p;  // time in units of one unsplit tile
       const double cost = waves * s.kt + 6.0 * (p > 1) + 0.15 * p;          // the join costs about six steps and grows with the parts
       if (cost < best - 1e-9) best = cost, s.splits = p;
     }
   }
   return s;
 }
-static int64_t part_ld(const GemmCall &c) { return (c.n + 3) / 4 * 4 * (c.dual == DUAL_GATED ? 2 : 1); }
+static int64_t part_ld(const GemmCall &c) { return (c.n + 3) / 4 * 4 * (paired(c) ? 2 : 1); }
 
 int64_t gemm_workspace_bytes(const GemmCall &c) {
   if (c.m <= 0 || c.n <= 0 || c.k <= 0) return 0;
@@ -667,34 +844,51 @@ int64_t gemm_workspace_bytes(const GemmCall &c) {
   return s.splits > 1 ? (int64_t)s.splits * s.batch * c.m * part_ld(c) * (int64_t)sizeof(float) : 0;
 }
 
-template <int BN, bool FP8, bool GATED> static int run(const GemmArgs &a, int grid, cudaStream_t stream) {
+template <int BN, int CTAS, bool FP8, int MODE> static int run(const GemmArgs &a, int sms, cudaStream_t stream) {
   // a per-device attribute of the function: set on every call (a process may use several GPUs)
-  GPHL_CUDA(cudaFuncSetAttribute(gemm_kernel<BN, FP8, GATED>, cudaFuncAttributeMaxDynamicSharedMemorySize, GEMM_SMEM));
-  gemm_kernel<BN, FP8, GATED><<<grid, GEMM_THREADS, GEMM_SMEM, stream>>>(a);
+  GPHL_CUDA(cudaFuncSetAttribute(gemm_kernel<BN, CTAS, FP8, MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, GEMM_SMEM));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(std::min<int64_t>(a.work, sms / CTAS) * CTAS)), cfg.blockDim = dim3(GEMM_THREADS);
+  cfg.dynamicSmemBytes = GEMM_SMEM, cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CTAS, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr, cfg.numAttrs = CTAS > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, gemm_kernel<BN, CTAS, FP8, MODE>, a);
   return launched("gemm_kernel");
+}
+template <bool FP8, int MODE> static int run_shape(const Shape &s, const GemmArgs &a, int sms, cudaStream_t stream) {
+  if (s.ctas == 2) return run<256, 2, FP8, MODE>(a, sms, stream);
+  if (s.bn == 256) return run<256, 1, FP8, MODE>(a, sms, stream);
+  if constexpr (MODE == LINEAR)
+    if (s.bn == 64) return run<64, 1, FP8, MODE>(a, sms, stream);
+  return run<128, 1, FP8, MODE>(a, sms, stream);
 }
 
 int gemm(const GemmCall &c, const char *what, cudaStream_t stream) {
   if (!encode_fn()) return fail(GPHL_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", what);
   const Shape s = shape_of(c);
-  const bool gated = c.dual == DUAL_GATED;
+  const bool pairs_of_b = paired(c);
   GemmArgs a{};
   const int pairs = c.dual == DUAL_NONE ? 1 : 2;
   for (int i = 0; i < pairs; ++i) {
-    if (i == 0 || !gated) {
+    if (i == 0 || !pairs_of_b) {
       int rc = encode(&a.a[i], c.a[i], c.in_type, c.fp8, c.a_mn ? 64 : GM, what);
       if (rc != GPHL_OK) return rc;
     }
-    int rc = encode(&a.b[i], c.b[i], c.in_type, c.fp8, c.b_mn ? 64 : gated ? s.bn / 2 : s.bn, what);
+    int rc = encode(&a.b[i], c.b[i], c.in_type, c.fp8, c.b_mn ? 64 : pairs_of_b ? s.bn / 2 : s.bn / s.ctas, what);
     if (rc != GPHL_OK) return rc;
   }
-  a.m = c.m, a.n = c.n, a.tiles_m = s.tiles_m, a.tiles_n = s.tiles_n, a.work = s.tiles_m * s.tiles_n * s.batch * s.splits;
+  const int64_t work = s.tiles_m * s.tiles_n * s.batch * s.splits;
+  GPHL_REQUIRE(work + 65536 < INT32_MAX, "%s: too many tiles", what);
+  a.m = c.m, a.n = c.n, a.tiles_m = (uint32_t)s.tiles_m, a.tiles_n = (uint32_t)s.tiles_n, a.work = (uint32_t)work;
   a.batch = s.batch, a.splits = s.splits, a.kt = s.kt, a.kt_first = c.dual == DUAL_CONCAT ? s.kt / 2 : s.kt;
   a.a_mn = c.a_mn, a.b_mn = c.b_mn, a.types = (int32_t)c.types, a.ptr = c.ptr;
-  a.idesc = (1u << 4) | ((uint32_t)(s.bn >> 3) << 17) | ((uint32_t)(GM >> 4) << 24);
+  a.idesc = (1u << 4) | ((uint32_t)(s.bn >> 3) << 17) | ((uint32_t)(GM * s.ctas >> 4) << 24);
   if (!c.fp8) a.idesc |= (c.in_type == GPHL_BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)c.a_mn << 15) | ((uint32_t)c.b_mn << 16);
   a.out[0] = c.out[0], a.out[1] = c.out[1], a.ld_out = c.ld_out, a.out_type = c.out_type, a.act = c.act;
   a.out_vec = aligned16(c.out[0]) && aligned16(c.out[1]) && (c.ld_out * (c.out_type == GPHL_F32 ? 4 : 2)) % 16 == 0;
+  a.dh = c.dh, a.dh_vec = aligned16(c.dh) && c.n % 8 == 0;
   a.g = c.g, a.u = c.u, a.ld_gu = c.ld_gu, a.q = c.q, a.q_scale = c.q_scale, a.q_scale_stride = c.q_scale_stride;
   a.part = static_cast<float *>(c.workspace), a.ld_part = part_ld(c), a.part_u = (c.n + 3) / 4 * 4;
   a.a_scale = c.a_scale, a.b_scale[0] = c.b_scale[0], a.b_scale[1] = c.b_scale[1];
@@ -704,19 +898,15 @@ int gemm(const GemmCall &c, const char *what, cudaStream_t stream) {
   int dev = 0, sms = 0;
   GPHL_CUDA(cudaGetDevice(&dev));
   GPHL_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-  const int grid = (int)std::min<int64_t>(a.work, sms);
   int rc;
-  if (c.fp8) {
-    if (gated) rc = s.bn == 256 ? run<256, true, true>(a, grid, stream) : run<128, true, true>(a, grid, stream);
-    else rc = s.bn == 256 ? run<256, true, false>(a, grid, stream) : s.bn == 128 ? run<128, true, false>(a, grid, stream) : run<64, true, false>(a, grid, stream);
-  } else {
-    if (gated) rc = s.bn == 256 ? run<256, false, true>(a, grid, stream) : run<128, false, true>(a, grid, stream);
-    else rc = s.bn == 256 ? run<256, false, false>(a, grid, stream) : s.bn == 128 ? run<128, false, false>(a, grid, stream) : run<64, false, false>(a, grid, stream);
-  }
+  if (c.dual == DUAL_GATED_GRAD) rc = run_shape<false, GATED_GRAD>(s, a, sms, stream);
+  else if (c.dual == DUAL_GATED) rc = c.fp8 ? run_shape<true, GATED>(s, a, sms, stream) : run_shape<false, GATED>(s, a, sms, stream);
+  else rc = c.fp8 ? run_shape<true, LINEAR>(s, a, sms, stream) : run_shape<false, LINEAR>(s, a, sms, stream);
   if (rc != GPHL_OK || s.splits == 1) return rc;
-  const int64_t items = s.batch * c.m * ((c.n + 127) / 128);
-  if (gated) gemm_join_kernel<true><<<(unsigned)((items + 7) / 8), 256, 0, stream>>>(a);
-  else gemm_join_kernel<false><<<(unsigned)((items + 7) / 8), 256, 0, stream>>>(a);
+  const unsigned blocks = (unsigned)((s.batch * c.m * ((c.n + 127) / 128) + 7) / 8);
+  if (c.dual == DUAL_GATED_GRAD) gemm_join_kernel<GATED_GRAD><<<blocks, 256, 0, stream>>>(a);
+  else if (c.dual == DUAL_GATED) gemm_join_kernel<GATED><<<blocks, 256, 0, stream>>>(a);
+  else gemm_join_kernel<LINEAR><<<blocks, 256, 0, stream>>>(a);
   return launched("gemm_join_kernel");
 }
 

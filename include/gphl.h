@@ -345,6 +345,7 @@ int64_t gphl_gated_workspace_bytes(int64_t m, int64_t k, int64_t f);
 int gphl_gated(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t f, const void *x, int64_t ldx, const void *wg, const void *wu,
                int64_t ldw, int32_t w_transposed, void *h, float *g, float *u, int64_t ld_gu, void *workspace, void *stream);
 /* Its backward pass: dg = dh u act'(g), du = dh act(g) (rounded to dtype), dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du.
+ * g and u as gphl_gated stored them, or both NULL: they are made again from x and the weights.
  * dx (m, k) and dWg, dWu (laid out as the weights, contiguous) may each be NULL when not wanted (the two weights' together). */
 int64_t gphl_gated_grad_workspace_bytes(int64_t m, int64_t k, int64_t f);
 int gphl_gated_grad(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t f, const void *dh, const float *g, const float *u, int64_t ld_gu,

@@ -168,7 +168,8 @@ def check_mm(x, w, ptr, dtype, out=None):
 
 
 @pytest.mark.parametrize("m,k,n", [(1, 1, 1), (1, 128, 128), (1, 16, 24), (2, 200, 65), (128, 128, 256), (129, 384, 300), (100, 1000, 777), (1, 4096, 4096),
-                                   (7, 2048, 1000), (1000, 640, 1500), (300, 5000, 64), (4096, 256, 512), (640, 129, 20000)])
+                                   (7, 2048, 1000), (1000, 640, 1500), (300, 5000, 64), (4096, 256, 512), (640, 129, 20000),
+                                   (5000, 500, 2100), (260, 2000, 3000)])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_mm_fp8(m, k, n, dtype):
     check_mm(codes(m, k, 10), weights(1, k, n, 20), None, dtype)
@@ -181,6 +182,10 @@ def test_mm_fp8_typed(ptr, k, n):
     out = torch.full((m, n), 7.0, device="cuda", dtype=BF16)
     y = check_mm(codes(m, k, 10), weights(4, k, n, 20), ptr, BF16, out=out)
     assert y is out and (out[:ptr[0]] == 7).all() and (out[ptr[-1]:] == 7).all()      # rows of no type stay
+
+
+def test_mm_fp8_long_types():
+    check_mm(codes(4100, 300, 10), weights(3, 300, 2100, 20), [0, 1500, 1500, 4100], BF16)
 
 
 def test_mm_fp8_many_types():
@@ -214,7 +219,7 @@ def test_mm_fp8_nan_stays_in_its_row():
 # ---- gated feed-forward ---------------------------------------------------------------------------------------------
 
 GATED_SHAPES = [(1, 1, 1), (1, 64, 64), (3, 7, 9), (2, 8, 130), (128, 64, 128), (129, 200, 136), (100, 1001, 77), (1, 2048, 1024), (5, 520, 1400),
-                (700, 96, 264), (2000, 256, 320)]
+                (700, 96, 264), (2000, 256, 320), (3000, 264, 1000), (1300, 2056, 400)]
 
 
 def gated_inputs(m, k, f, dtype, transposed):
@@ -255,13 +260,15 @@ def test_gated_grad(m, k, f, dtype, transposed, act):
     got = c.gated_linear_grad(dh, g, u, x, wg, wu, act)
     for name, a, (want, err) in zip(("dx", "dwg", "dwu"), got, ref.gated_grad(dh, x, wg, wu, act, dtype)):
         ref.close(a, want, err, what=name)
+    for name, a, (want, err) in zip(("dx", "dwg", "dwu"), c.gated_linear_grad(dh, None, None, x, wg, wu, act), ref.gated_grad(dh, x, wg, wu, act, dtype)):
+        ref.close(a, want, err, what=name + " with the projections made again")
     only = c.gated_linear_grad(dh, g, u, x, wg, wu, act, want_dw=False)
     assert torch.equal(only[0], got[0]) and only[1] is None
     only = c.gated_linear_grad(dh, g, u, x, wg, wu, act, want_dx=False)
     assert only[0] is None and torch.equal(only[1], got[1]) and torch.equal(only[2], got[2])
 
 
-@pytest.mark.parametrize("m,k,f", [(1, 128, 128), (1, 4096, 1000), (3, 200, 65), (129, 384, 300), (300, 1000, 777), (2000, 256, 640)])
+@pytest.mark.parametrize("m,k,f", [(1, 128, 128), (1, 4096, 1000), (3, 200, 65), (129, 384, 300), (300, 1000, 777), (2000, 256, 640), (2500, 300, 1200)])
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16, torch.float8_e4m3fn])
 def test_gated_fp8(m, k, f, act, dtype):
