@@ -55,18 +55,31 @@ int gemm_wait_timeouts(int *count);
 int gemm_reset_wait_timeouts();
 
 #ifdef __CUDACC__
+// One instruction each (2 units in the last place): division and exponential would cost several.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float LOG2E = 1.4426950408889634f;
+__device__ __forceinline__ float sigmoid_fast(float g) { return rcp_fast(1.f + exp2_fast(-LOG2E * g)); }
 // Phi(g), and exp(-g^2 / 2) by the way: Phi(-x) = P(t) exp(-x^2 / 2) / 2, t = 1 / (1 + 0.3275911 x / sqrt 2), the rational
 // approximation 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions for erf (absolute error 1.5e-7); the tail keeps
 // its leading digits, which 1 + erf does not.
 __device__ __forceinline__ float normal_cdf(float g, float &e) {
-  const float x = fabsf(g) * 0.70710678118654752f, t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-  e = __expf(-x * x);
+  const float t = rcp_fast(fmaf(0.3275911f * 0.70710678118654752f, fabsf(g), 1.f));
+  e = exp2_fast(-0.5f * LOG2E * g * g);
   const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
   const float tail = 0.5f * p * e;
   return g < 0.f ? tail : 1.f - tail;
 }
 template <int ACT> __device__ __forceinline__ float activate(float g) {
-  if constexpr (ACT == ACT_SILU) return __fdividef(g, 1.f + __expf(-g));
+  if constexpr (ACT == ACT_SILU) return g * sigmoid_fast(g);
   if constexpr (ACT == ACT_GELU) {
     float e;
     return g * normal_cdf(g, e);
@@ -77,8 +90,8 @@ template <int ACT> __device__ __forceinline__ float activate(float g) {
 template <int ACT> __device__ __forceinline__ void gate_grads(float dh, float &g, float &u) {
   float h, d;                                      // act(g) and act'(g)
   if constexpr (ACT == ACT_SILU) {
-    const float s = __fdividef(1.f, 1.f + __expf(-g));
-    h = g * s, d = s * (1.f + g * (1.f - s));
+    const float s = sigmoid_fast(g);
+    h = g * s, d = fmaf(h, 1.f - s, s);
   } else if constexpr (ACT == ACT_GELU) {
     float e;
     const float c = normal_cdf(g, e);
