@@ -622,7 +622,7 @@ def rms_norm_grad(r, weight, rstd, dy, dr=None):
 
 
 def rms_norm_fp8(x, weight, eps: float = 1e-6, residual=None):
-    """``rms_norm`` with y in 8 bits (``Fp8Rows``), each code the correct rounding of the normalised value; scales are powers of two.
+    """``rms_norm`` with y in 8 bits (``Fp8Rows``), rounded once, from the float32 value; scales are powers of two.
     Returns y, or (y, r) with a residual."""
     out = _call("rms_norm_fp8", x, weight, eps, residual)
     y = Fp8Rows(out[0], out[1])

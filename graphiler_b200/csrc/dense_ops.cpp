@@ -20,9 +20,10 @@ using torch::autograd::variable_list;
 using OptTensor = c10::optional<Tensor>;
 
 constexpr int64_t BLOCK = 128;        // values of one 8-bit scale
-// Rows narrower than this keep no projections for the backward pass of the gated feed-forward: making g and u again costs 4 k operations
-// an element, storing and reading them 16 bytes.  One step of 300,000 x 256 -> 1024: see gated.cu for both sides measured.
-constexpr int64_t RECOMPUTE_K = 1024;
+// Rows of at most this width keep no projections for the backward pass of the gated feed-forward: making g and u again costs 4 k operations
+// an element, storing and reading them 16 bytes.  A step in bf16, made again / kept: 300,000 x 256 -> 1024 1.40 / 1.74 ms, 100,000 x 1024 ->
+// 1024 1.35 / 1.27 ms.
+constexpr int64_t RECOMPUTE_K = 768;
 
 int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 void check_rc(int rc, const char *what) { TORCH_CHECK(rc == GPHL_OK, what, " failed (", rc, "): ", gphl_last_error()); }

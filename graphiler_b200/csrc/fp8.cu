@@ -1,6 +1,6 @@
 // e4m3 rows and weights with a scale per block of 128, and the typed product of the two.
 //
-// The quantisers read every value once: a warp per (row, step) for rows, a block per 128 x 128 tile for weights, which turns the
+// The quantisers read every value once: a few steps of a row a warp, a block per 128 x 128 tile for weights, which turns the
 // tile round in shared memory (segment_mm's weights have n contiguous, the product reads k contiguous).  Scales are powers of two, so that
 // scaling rounds nothing and a code is the rounding of the value itself.
 #include <algorithm>
@@ -10,27 +10,24 @@
 
 namespace gphl {
 
-template <typename T, bool SC>
+// NV steps of a row a warp (32 / LPR rows), all loads first.
+template <typename T, typename R, int NV>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T *__restrict__ x, int64_t m, int32_t n, uint8_t *__restrict__ q, int32_t n_pad,
                                                             float *__restrict__ scales, int64_t scale_stride) {
-  using R = Row<T, SC>;
-  constexpr int E = R::E, LANES = 128 / E;
-  const int lane = threadIdx.x & 31, steps = (n + R::STEP - 1) / R::STEP;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), row = item / steps;
-  const int step = (int)(item - row * steps);
-  if (row >= m) return;
-  float v[E], big = 0.f;
-  R::load(x + row * n, step, lane, n, v);
+  constexpr int RPW = 32 / R::LPR;
+  const int lane = threadIdx.x & (R::LPR - 1), groups = (n + R::STEP * NV - 1) / (R::STEP * NV);
+  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), first = item / groups;
+  const int step0 = (int)(item - first * groups) * NV;
+  const int64_t at = first * RPW + (threadIdx.x & 31) / R::LPR, row = min(at, m - 1);      // rows past the last store nothing
+  typename R::Raw v[NV];
 #pragma unroll
-  for (int j = 0; j < E; ++j) big = fmaxf(big, finite_abs(v[j]));
-  const int e = fp8_exponent(block_max<T, SC>(big));
-  const float inv = pow2f(-e);
-  uint32_t c[E];
+  for (int i = 0; i < NV; ++i) v[i] = R::raw(x + row * n, step0 + i, lane, n);
 #pragma unroll
-  for (int j = 0; j < E; ++j) c[j] = e4m3(v[j] * inv);
-  store_codes<T, SC>(q + row * n_pad, step, lane, n, n_pad, c);
-  const int block = R::col(step, lane, 0) / 128;
-  if (lane % LANES == 0 && block * 128 < n) scales[block * scale_stride + row] = pow2f(e);
+  for (int i = 0; i < NV; ++i) {
+    float y[R::E];
+    R::widen(v[i], y);
+    if (i == 0 || (step0 + i) * R::STEP < n_pad) store_codes<R>(y, q + row * n_pad, scales + row, scale_stride, step0 + i, lane, n, n_pad, at < m);
+  }
 }
 
 constexpr int TILE_LD = 132;                          // bytes from n to n in shared memory: 4 more than a row, so that stores spread over the banks
@@ -71,35 +68,38 @@ __global__ void __launch_bounds__(256) quantize_weight_kernel(const T *__restric
       *reinterpret_cast<uint32_t *>(q + (t * n + n0 + r) * k_stride + k0 + lane * 4) = tile[r * (TILE_LD / 4) + lane];
 }
 
-// A warp per (row, 512 columns), 16 codes a lane; rows of codes start on 16-byte boundaries.
-template <typename T>
+// Rows of codes start on 16-byte boundaries.  VEC: a thread per 16 neighbouring codes.  Otherwise a warp per 512 columns of a row, columns 32
+// apart, so that stores to rows of any width and base are still whole lines.
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t *__restrict__ q, int64_t q_stride, const float *__restrict__ scales,
-                                                         int64_t row_stride, int64_t block_stride, int64_t m, int32_t n, T *__restrict__ y, bool vec) {
-  const int lane = threadIdx.x & 31, steps = (n + 511) / 512;
-  const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), row = item / steps;
-  const int c0 = (int)(item - row * steps) * 512 + lane * 16;
-  if (row >= m || c0 >= n) return;
-  const float s = __ldg(scales + row * row_stride + (c0 / 128) * block_stride);
-  uint8_t code[16];
-  if (c0 + 16 <= n) {
-    *reinterpret_cast<uint4 *>(code) = *reinterpret_cast<const uint4 *>(q + row * q_stride + c0);
+                                                         int64_t row_stride, int64_t block_stride, int64_t m, int32_t n, T *__restrict__ y) {
+  auto value = [](uint8_t code) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3))); };
+  if constexpr (VEC) {
+    const int64_t units = (n + 15) / 16, i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / units;
+    const int c0 = (int)(i - row * units) * 16;        // n is a multiple of 8
+    if (row >= m) return;
+    const uint8_t *src = q + row * q_stride + c0;
+    const float s = __ldg(scales + row * row_stride + (c0 / 128) * block_stride);
+    __align__(16) uint8_t code[16];
+    if (c0 + 16 <= n) *reinterpret_cast<uint4 *>(code) = *reinterpret_cast<const uint4 *>(src);
+    else *reinterpret_cast<uint2 *>(code) = *reinterpret_cast<const uint2 *>(src);
+    __align__(16) T out[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) out[j] = from_float<T>(c0 + j < n ? value(code[j]) * s : 0.f);
+    T *dst = y + row * n + c0;
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T); ++j)
+      if (c0 + (j + 1) * 16 / (int)sizeof(T) <= n) reinterpret_cast<uint4 *>(dst)[j] = reinterpret_cast<const uint4 *>(out)[j];
   } else {
-    for (int j = 0; j < 16; ++j) code[j] = c0 + j < n ? q[row * q_stride + c0 + j] : (uint8_t)0;
-  }
-  T out[16];
+    const int lane = threadIdx.x & 31, steps = (n + 511) / 512;
+    const int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), row = item / steps;
+    const int base = (int)(item - row * steps) * 512;
+    if (row >= m) return;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const __half_raw h = __nv_cvt_fp8_to_halfraw(code[j], __NV_E4M3);
-    out[j] = from_float<T>(__half2float(__half(h)) * s);
-  }
-  T *dst = y + row * n + c0;
-  if (vec && c0 + 16 <= n) {
-#pragma unroll
-    for (int j = 0; j < (int)sizeof(T); ++j) reinterpret_cast<uint4 *>(dst)[j] = reinterpret_cast<const uint4 *>(out)[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-      if (c0 + j < n) dst[j] = out[j];
+    for (int j = 0; j < 16; ++j) {
+      const int c = base + lane + 32 * j;
+      if (c < n) y[row * n + c] = from_float<T>(value(q[row * q_stride + c]) * __ldg(scales + row * row_stride + (c / 128) * block_stride));
+    }
   }
 }
 
@@ -117,10 +117,28 @@ static bool known(int dtype) { return dtype >= GPHL_F32 && dtype <= GPHL_F16; }
 
 template <typename T> static void quantize(const void *x, int64_t m, int64_t n, void *q, int64_t n_pad, float *scales, int64_t stride, cudaStream_t s) {
   const bool vec = aligned16(x) && n % (16 / (int)sizeof(T)) == 0;
-  const int64_t steps = vec ? (n + Row<T, false>::STEP - 1) / Row<T, false>::STEP : (n + 127) / 128;
-  const unsigned grid = (unsigned)((m * steps + 7) / 8);
-  if (vec) quantize_rows_kernel<T, false><<<grid, 256, 0, s>>>(static_cast<const T *>(x), m, (int32_t)n, static_cast<uint8_t *>(q), (int32_t)n_pad, scales, stride);
-  else quantize_rows_kernel<T, true><<<grid, 256, 0, s>>>(static_cast<const T *>(x), m, (int32_t)n, static_cast<uint8_t *>(q), (int32_t)n_pad, scales, stride);
+  with_lanes<T>(n, vec, [&](auto r) {
+    using R = decltype(r);
+    auto launch = [&](auto nv) {
+      constexpr int RPW = 32 / R::LPR, NV = decltype(nv)::value;
+      const int64_t items = ((m + RPW - 1) / RPW) * ((n + R::STEP * NV - 1) / (R::STEP * NV));
+      quantize_rows_kernel<T, R, NV><<<(unsigned)((items + 7) / 8), 256, 0, s>>>(static_cast<const T *>(x), m, (int32_t)n, static_cast<uint8_t *>(q),
+                                                                                (int32_t)n_pad, scales, stride);
+    };
+    // several loads under way per lane where rows have them (32768 x 8192 in bf16: 148 against 253 us)
+    if constexpr (R::LPR == 32) {
+      if (n > 2 * R::STEP) return launch(std::integral_constant<int, 4>());
+    }
+    launch(std::integral_constant<int, 1>());
+  });
+}
+template <typename T>
+static void dequantize(const void *q, int64_t q_stride, const float *scales, int64_t row_stride, int64_t block_stride, int64_t m, int64_t n, void *y, cudaStream_t s) {
+  if (aligned16(y) && n % 8 == 0)
+    dequantize_kernel<T, true><<<(unsigned)((m * ((n + 15) / 16) + 255) / 256), 256, 0, s>>>(static_cast<const uint8_t *>(q), q_stride, scales, row_stride, block_stride,
+                                                                                            m, (int32_t)n, static_cast<T *>(y));
+  else
+    dequantize_kernel<T, false><<<(unsigned)((m * ((n + 511) / 512) + 7) / 8), 256, 0, s>>>(static_cast<const uint8_t *>(q), q_stride, scales, row_stride, block_stride, m, (int32_t)n, static_cast<T *>(y));
 }
 
 }  // namespace gphl
@@ -169,13 +187,9 @@ extern "C" int gphl_dequantize_fp8(int32_t dtype, int64_t m, int64_t n, const vo
   GPHL_REQUIRE(q && scales && y, "null pointer argument");
   GPHL_REQUIRE(q_stride >= n && q_stride % 16 == 0 && aligned16(q), "dequantize_fp8: code rows must start on 16-byte boundaries");
   cudaStream_t s = static_cast<cudaStream_t>(stream_);
-  const unsigned grid = (unsigned)((m * ((n + 511) / 512) + 7) / 8);
-  const uint8_t *c = static_cast<const uint8_t *>(q);
-  const bool vec = aligned16(y) && n % 8 == 0;
-  if (dtype == GPHL_F32) dequantize_kernel<float><<<grid, 256, 0, s>>>(c, q_stride, scales, scale_row_stride, scale_block_stride, m, (int32_t)n, static_cast<float *>(y), vec);
-  else if (dtype == GPHL_BF16)
-    dequantize_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(c, q_stride, scales, scale_row_stride, scale_block_stride, m, (int32_t)n, static_cast<__nv_bfloat16 *>(y), vec);
-  else dequantize_kernel<__half><<<grid, 256, 0, s>>>(c, q_stride, scales, scale_row_stride, scale_block_stride, m, (int32_t)n, static_cast<__half *>(y), vec);
+  if (dtype == GPHL_F32) dequantize<float>(q, q_stride, scales, scale_row_stride, scale_block_stride, m, n, y, s);
+  else if (dtype == GPHL_BF16) dequantize<__nv_bfloat16>(q, q_stride, scales, scale_row_stride, scale_block_stride, m, n, y, s);
+  else dequantize<__half>(q, q_stride, scales, scale_row_stride, scale_block_stride, m, n, y, s);
   return launched("dequantize_kernel");
 }
 

@@ -4,8 +4,10 @@
 // y in the rows' type, or as e4m3 codes with one power-of-two scale per row and block of 128 columns.  Backward, from r and rstd:
 //   g = dy * w, xhat = r * rstd, dx = dr + rstd * (g - xhat * mean(g * xhat)), dw = sum over rows of dy * xhat.
 //
-// Memory bound.  A row is read once and stays in registers: WPR warps hold it, up to NV steps each (a step is 32 lanes x 16 bytes); the
-// sum of squares is kept in fp32 by every lane (at most 32 terms) and joined in double.  Rows too wide for that are read twice.
+// Memory bound.  A row is read once and stays in registers: WPR warps hold it, up to NV steps each (a step is 32 lanes x 16 bytes).  Sums
+// of a row are fp32: at most 32 terms a lane, then a tree over lanes and warps, so an error of a few 2^-24.  (Joining them and taking the
+// root in double was the bound of short rows: 600,000 x 256 in bf16 took 251 us forward and 429 us backward.)  Rows too wide for the
+// registers are read twice.
 #include <algorithm>
 #include <initializer_list>
 
@@ -24,48 +26,38 @@ struct NormArgs {
   float eps;
 };
 
-// Joins `v` over the warps of a row (all threads of the block when wpr > 1).
-__device__ __forceinline__ double row_sum(double v, int wpr, int warp, int lane, double *s_part) {
+// Joins `v` over the lanes of a row, or (wpr > 1) over its warps: all threads of the block.
+template <int LPR> __device__ __forceinline__ float row_sum(float v, int wpr, int warp, int lane, float *s_part) {
 #pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(FULL, v, d);
-  if (wpr == 1) return v;
+  for (int d = LPR / 2; d >= 1; d >>= 1) v += __shfl_xor_sync(FULL, v, d);
+  if (LPR < 32 || wpr == 1) return v;
   if (lane == 0) s_part[warp] = v;
   __syncthreads();
-  v = lane < wpr ? s_part[lane] : 0.0;
+  v = lane < wpr ? s_part[lane] : 0.f;
 #pragma unroll
   for (int d = 16; d >= 1; d >>= 1) v += __shfl_xor_sync(FULL, v, d);
   __syncthreads();                                   // s_part may be written again
   return v;
 }
 
-// Correct rounding of v * w * rstd / scale to e4m3 where the fp32 value is too close to a border between two codes: the product in
-// double, brought to fp32 by rounding to odd, which leaves the second rounding unbiased.
-__device__ __noinline__ uint32_t e4m3_near_border(float v, float w, double rstd, float inv) {
-  const double t = (double)v * (double)w * rstd * (double)inv;
-  float f = __double2float_rz(t);
-  if ((double)f != t) f = __uint_as_float(__float_as_uint(f) | 1u);
-  return e4m3(f);
-}
-
 // NV > 0: the row is held in registers.  NV == 0: any width, the row is read twice.
-template <typename T, bool SC, int NV, bool FP8>
+template <typename T, typename R, int NV, bool FP8>
 __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
-  using R = Row<T, SC>;
-  constexpr int E = R::E;
-  __shared__ double s_part[16];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per_block = (blockDim.x >> 5) / a.wpr;   // rows of a block: several one-warp rows, or one row
-  const int64_t row = (int64_t)blockIdx.x * per_block + warp / a.wpr;
-  if (row >= a.m) return;                            // whole warps, and only in blocks of one-warp rows
+  constexpr int E = R::E, RPW = 32 / R::LPR;         // rows of a warp
+  __shared__ float s_part[16];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & (R::LPR - 1);
+  const int per_block = (blockDim.x >> 5) / a.wpr * RPW;
+  // rows past the last one do the last one's work over again and store nothing: all lanes of a warp take part in its shuffles
+  const int64_t at = (int64_t)blockIdx.x * per_block + (warp / a.wpr) * RPW + (threadIdx.x & 31) / R::LPR, row = min(at, a.m - 1);
+  const bool live = at < a.m;
   const int w0 = warp % a.wpr, steps = (a.n + R::STEP - 1) / R::STEP;
   const T *x = static_cast<const T *>(a.x) + row * a.n;
   const T *res = a.res ? static_cast<const T *>(a.res) + row * a.n : nullptr;
-  T *r = a.r ? static_cast<T *>(a.r) + row * a.n : nullptr;
+  T *r = a.r && live ? static_cast<T *>(a.r) + row * a.n : nullptr;
 
   constexpr int KEEP = NV > 0 ? NV : 1;
   float v[KEEP][E];
   float ss = 0.f;
-  double wide = 0.0;
   auto read = [&](int step, float (&t)[E]) {
     R::load(x, step, lane, a.n, t);
     if (res) {
@@ -90,20 +82,18 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
         for (int j = 0; j < E; ++j) ss = fmaf(v[i][j], v[i][j], ss);
       }
     }
-    wide = (double)ss;
   } else {
     for (int step = w0; step < steps; step += a.wpr) {
       read(step, v[0]);
       if (r) R::store(r, step, lane, a.n, v[0]);
-      ss = 0.f;
+      float part = 0.f;
 #pragma unroll
-      for (int j = 0; j < E; ++j) ss = fmaf(v[0][j], v[0][j], ss);
-      wide += (double)ss;
+      for (int j = 0; j < E; ++j) part = fmaf(v[0][j], v[0][j], part);
+      ss += part;
     }
   }
-  const double rstd_d = 1.0 / sqrt(row_sum(wide, a.wpr, warp, lane, s_part) / a.n + (double)a.eps);
-  const float rstd = (float)rstd_d;
-  if (a.rstd && w0 == 0 && lane == 0) a.rstd[row] = rstd;
+  const float rstd = 1.f / sqrtf(row_sum<R::LPR>(ss, a.wpr, warp, lane, s_part) / (float)a.n + a.eps);
+  if (a.rstd && w0 == 0 && lane == 0 && live) a.rstd[row] = rstd;
 
   auto write = [&](int step, const float (&t)[E]) {
     float w[E], y[E];
@@ -111,32 +101,8 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
     else R::load(static_cast<const T *>(a.w), step, lane, a.n, w);
 #pragma unroll
     for (int j = 0; j < E; ++j) y[j] = t[j] * rstd * w[j];
-    if constexpr (FP8) {
-      float big = 0.f;
-#pragma unroll
-      for (int j = 0; j < E; ++j) big = fmaxf(big, finite_abs(y[j]));
-      const int e = fp8_exponent(block_max<T, SC>(big));
-      const float inv = pow2f(-e);
-      uint32_t q[E];
-#pragma unroll
-      for (int j = 0; j < E; j += 2) {
-        // y carries three fp32 roundings (at most 3 x 2^-24 relative): if both ends of a wider interval have one code, it is the code
-        const float s0 = y[j] * inv, s1 = y[j + 1] * inv;
-        const uint32_t up = e4m3x2(s0 * (1.f + 0x1p-21f), s1 * (1.f + 0x1p-21f));
-        const uint32_t dn = e4m3x2(s0 * (1.f - 0x1p-21f), s1 * (1.f - 0x1p-21f));
-        q[j] = up & 0xff, q[j + 1] = up >> 8;
-        if (up != dn) {
-          q[j] = e4m3_near_border(t[j], w[j], rstd_d, inv);
-          q[j + 1] = e4m3_near_border(t[j + 1], w[j + 1], rstd_d, inv);
-        }
-      }
-      store_codes<T, SC>(a.q + row * a.n_pad, step, lane, a.n, a.n_pad, q);
-      constexpr int LANES = 128 / E;
-      const int block = R::col(step, lane, 0) / 128;
-      if (lane % LANES == 0 && block * 128 < a.n) a.scales[block * a.scale_stride + row] = pow2f(e);
-    } else {
-      R::store(static_cast<T *>(a.y) + row * a.n, step, lane, a.n, y);
-    }
+    if constexpr (FP8) store_codes<R>(y, a.q + row * a.n_pad, a.scales + row, a.scale_stride, step, lane, a.n, a.n_pad, live);
+    else if (live) R::store(static_cast<T *>(a.y) + row * a.n, step, lane, a.n, y);
   };
   if constexpr (NV > 0) {
 #pragma unroll
@@ -163,65 +129,83 @@ struct NormGradArgs {
 };
 
 // Rows are dealt to warps (or, for wpr > 1, to blocks) in turn; a lane keeps its columns, so dw gathers in its registers over all the
-// rows it meets and leaves once.  The rows' sums g.xhat are joined in double.
-template <typename T, bool SC, int NV>
-__global__ void __launch_bounds__(512) rms_norm_grad_kernel(const NormGradArgs a) {
-  using R = Row<T, SC>;
-  constexpr int E = R::E;
-  __shared__ double s_part[16];
-  extern __shared__ float s_dw[];                    // wpr == 1: one row of n sums per warp
-  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per_block = warps / a.wpr, w0 = warp % a.wpr, steps = (a.n + R::STEP - 1) / R::STEP;
+// rows it meets and leaves once.  The next row's r and dy are on their way while a row is finished, and a lane holds 8 values of each, so
+// that 32 warps fit an SM.
+template <typename T, typename R>
+__global__ void __launch_bounds__(1024) rms_norm_grad_kernel(const NormGradArgs a) {
+  constexpr int E = R::E, NV = 8 / E, RPW = 32 / R::LPR;
+  __shared__ float s_part[32];
+  extern __shared__ float s_dw[];                    // wpr == 1: n sums per row slot of the block
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & (R::LPR - 1), sub = (threadIdx.x & 31) / R::LPR;
+  const int slots = warps / a.wpr * RPW, slot = (warp / a.wpr) * RPW + sub, w0 = warp % a.wpr, steps = (a.n + R::STEP - 1) / R::STEP;
   float dw[NV][E];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int j = 0; j < E; ++j) dw[i][j] = 0.f;
-  for (int64_t row = (int64_t)blockIdx.x * per_block + warp / a.wpr; row < a.m; row += (int64_t)gridDim.x * per_block) {
-    const T *r = static_cast<const T *>(a.r) + row * a.n, *dy = static_cast<const T *>(a.dy) + row * a.n;
-    const T *dr = a.dr ? static_cast<const T *>(a.dr) + row * a.n : nullptr;
-    const float rstd = __ldg(a.rstd + row);
-    float xh[NV][E], g[NV][E];
+  typename R::Raw r[NV], dy[NV];
+  float rstd = 0.f;
+  // past the last row: its values again, which count for nothing
+  auto fetch = [&](int64_t at) {
+    const int64_t row = min(at, a.m - 1);
+    rstd = __ldg(a.rstd + row);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int step = w0 + i * a.wpr;
       if (step < steps) {
-        R::load(r, step, lane, a.n, xh[i]);
-        R::load(dy, step, lane, a.n, g[i]);
+        r[i] = R::raw(static_cast<const T *>(a.r) + row * a.n, step, lane, a.n);
+        dy[i] = R::raw(static_cast<const T *>(a.dy) + row * a.n, step, lane, a.n);
       }
     }
-    double sum = 0.0;
+  };
+  const int64_t stride = (int64_t)gridDim.x * slots;
+  int64_t first = (int64_t)blockIdx.x * slots + (warp / a.wpr) * RPW;      // of the warp's rows: uniform in the warp
+  if (first < a.m) fetch(first + sub);
+  for (; first < a.m; first += stride) {
+    const int64_t row = first + sub;
+    const bool live = row < a.m;
+    float xh[NV][E], g[NV][E];
+    typename R::Raw dr[NV];
+    float sum = 0.f;
+    const float scale = rstd;
+    const int64_t at = min(row, a.m - 1) * a.n;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (a.dr && w0 + i * a.wpr < steps) dr[i] = R::raw(static_cast<const T *>(a.dr) + at, w0 + i * a.wpr, lane, a.n);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int step = w0 + i * a.wpr;
       if (step < steps) {
         float w[E], part = 0.f;
+        R::widen(r[i], xh[i]);
+        R::widen(dy[i], g[i]);
         if (a.w_f32) R::load(static_cast<const float *>(a.w), step, lane, a.n, w);
         else R::load(static_cast<const T *>(a.w), step, lane, a.n, w);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          xh[i][j] *= rstd;
-          dw[i][j] = fmaf(g[i][j], xh[i][j], dw[i][j]);
+          xh[i][j] *= scale;
+          if (RPW == 1 || live) dw[i][j] = fmaf(g[i][j], xh[i][j], dw[i][j]);
           g[i][j] *= w[j];
           part = fmaf(g[i][j], xh[i][j], part);
         }
-        sum += (double)part;
+        sum += part;
       }
     }
-    const float mean = (float)(row_sum(sum, a.wpr, warp, lane, s_part) / a.n);
-    T *dx = static_cast<T *>(a.dx) + row * a.n;
+    if (first + stride < a.m) fetch(row + stride);
+    const float mean = row_sum<R::LPR>(sum, a.wpr, warp, lane, s_part) / (float)a.n;
+    T *dx = static_cast<T *>(a.dx) + at;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int step = w0 + i * a.wpr;
       if (step < steps) {
         float o[E];
-        if (dr) R::load(dr, step, lane, a.n, o);
+        if (a.dr) R::widen(dr[i], o);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          const float t = rstd * fmaf(-xh[i][j], mean, g[i][j]);
-          o[j] = dr ? o[j] + t : t;
+          const float t = scale * fmaf(-xh[i][j], mean, g[i][j]);
+          o[j] = a.dr ? o[j] + t : t;
         }
-        R::store(dx, step, lane, a.n, o);
+        if (RPW == 1 || live) R::store(dx, step, lane, a.n, o);
       }
     }
   }
@@ -241,22 +225,21 @@ __global__ void __launch_bounds__(512) rms_norm_grad_kernel(const NormGradArgs a
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       const int c = R::col(i, lane, j);
-      if (c < a.n) s_dw[warp * a.n + c] = dw[i][j];
+      if (c < a.n) s_dw[slot * a.n + c] = dw[i][j];
     }
   __syncthreads();
   for (int c = threadIdx.x; c < a.n; c += blockDim.x) {
     float s = 0.f;
-    for (int k = 0; k < warps; ++k) s += s_dw[k * a.n + c];
+    for (int k = 0; k < slots; ++k) s += s_dw[k * a.n + c];
     part[c] = s;
   }
 }
 
-// Rows wider than the registers of 16 warps: one block per row reads its inputs twice; dw is left to rms_norm_dw_wide_kernel.
-template <typename T, bool SC>
+// Rows wider than the registers of 32 warps: one block per row reads its inputs twice; dw is left to rms_norm_dw_wide_kernel.
+template <typename T, typename R>
 __global__ void __launch_bounds__(512) rms_norm_grad_wide_kernel(const NormGradArgs a) {
-  using R = Row<T, SC>;
   constexpr int E = R::E;
-  __shared__ double s_part[16];
+  __shared__ float s_part[16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, steps = (a.n + R::STEP - 1) / R::STEP;
   const int64_t row = blockIdx.x;
   const T *r = static_cast<const T *>(a.r) + row * a.n, *dy = static_cast<const T *>(a.dy) + row * a.n;
@@ -272,15 +255,15 @@ __global__ void __launch_bounds__(512) rms_norm_grad_wide_kernel(const NormGradA
 #pragma unroll
     for (int j = 0; j < E; ++j) xh[j] *= rstd, g[j] *= w[j];
   };
-  double sum = 0.0;
+  float sum = 0.f;
   for (int step = warp; step < steps; step += a.wpr) {
     read(step);
     float part = 0.f;
 #pragma unroll
     for (int j = 0; j < E; ++j) part = fmaf(g[j], xh[j], part);
-    sum += (double)part;
+    sum += part;
   }
-  const float mean = (float)(row_sum(sum, a.wpr, warp, lane, s_part) / a.n);
+  const float mean = row_sum<32>(sum, a.wpr, warp, lane, s_part) / (float)a.n;
   for (int step = warp; step < steps; step += a.wpr) {
     read(step);
     float o[E];
@@ -305,18 +288,26 @@ __global__ void __launch_bounds__(256) rms_norm_dw_wide_kernel(const NormGradArg
   a.part[(int64_t)blockIdx.y * a.n + c] = s;
 }
 
-// dw = the partial sums' sum, in a fixed order, in double.
+// dw = the partial sums' sum, in a fixed order, in double: 32 threads a column, eight loads of each under way (with eight threads a column
+// and one load each, 2368 parts of 1001 columns took 42 us).
 template <typename T>
-__global__ void __launch_bounds__(256) rms_norm_dw_kernel(const float *__restrict__ part, int32_t parts, int32_t n, T *__restrict__ dw) {
-  __shared__ double s[8][33];
+__global__ void __launch_bounds__(1024) rms_norm_dw_kernel(const float *__restrict__ part, int32_t parts, int32_t n, T *__restrict__ dw) {
+  __shared__ double s[32][33];
   const int lane = threadIdx.x & 31, k0 = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   double v = 0.0;
-  if (c < n)
-    for (int k = k0; k < parts; k += 8) v += (double)part[(int64_t)k * n + c];
+  if (c < n) {
+    for (int k = k0; k < parts; k += 256) {
+      float t[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = k + 32 * j < parts ? __ldcs(part + (int64_t)(k + 32 * j) * n + c) : 0.f;
+      // fp32 pairs of neighbours in the tree, then double
+      v += (double)((t[0] + t[1]) + (t[2] + t[3])) + (double)((t[4] + t[5]) + (t[6] + t[7]));
+    }
+  }
   s[k0][lane] = v;
   __syncthreads();
   if (k0 == 0 && c < n) {
-    for (int k = 1; k < 8; ++k) v += s[k][lane];
+    for (int k = 1; k < 32; ++k) v += s[k][lane];
     dw[c] = from_float<T>((float)v);
   }
 }
@@ -327,29 +318,29 @@ static int pow2_at_least(int v) {
   return p;
 }
 
-template <typename T, bool SC, int NV, bool FP8> static void norm_launch(const NormArgs &a, int warps, cudaStream_t s) {
-  const int per_block = warps / a.wpr;
-  rms_norm_kernel<T, SC, NV, FP8><<<(unsigned)((a.m + per_block - 1) / per_block), warps * 32, 0, s>>>(a);
+template <typename T, typename R, int NV, bool FP8> static void norm_launch(const NormArgs &a, int warps, cudaStream_t s) {
+  const int per_block = warps / a.wpr * (32 / R::LPR);
+  rms_norm_kernel<T, R, NV, FP8><<<(unsigned)((a.m + per_block - 1) / per_block), warps * 32, 0, s>>>(a);
 }
-template <typename T, bool SC, bool FP8> static void norm_dispatch(NormArgs a, int sms, cudaStream_t s) {
-  using R = Row<T, SC>;
+template <typename T, typename R, bool FP8> static void norm_dispatch(NormArgs a, int sms, cudaStream_t s) {
   constexpr int LOW = 8 / R::E, HIGH = 32 / R::E;    // steps a warp holds: 8 or 32 values a lane
   const int steps = (a.n + R::STEP - 1) / R::STEP;
   // Few warps a row leave most loads in flight per warp and need the fewest joins; when the rows would not fill the GPU with 8 warps an
-  // SM that way, a row is spread over more warps instead (one row of 4096 columns, 16 bits: 2.3 us with 4 warps, 2.0 us with 16).
+  // SM that way, a row is spread over more warps instead.
   int wpr = pow2_at_least((steps + HIGH - 1) / HIGH);
-  const bool few = a.m * wpr < 8 * sms;
-  if (few) wpr = std::min(16, pow2_at_least((steps + LOW - 1) / LOW));
+  if (a.m * wpr < 8 * sms) wpr = pow2_at_least((steps + LOW - 1) / LOW);
   a.wpr = std::min(wpr, 16);
   const int warps = a.wpr == 1 ? 4 : a.wpr;
-  if (steps <= a.wpr * LOW) norm_launch<T, SC, LOW, FP8>(a, warps, s);
-  else if (steps <= a.wpr * HIGH) norm_launch<T, SC, HIGH, FP8>(a, warps, s);
-  else norm_launch<T, SC, 0, FP8>(a, warps, s);
+  if (steps <= a.wpr * LOW) norm_launch<T, R, LOW, FP8>(a, warps, s);
+  else if constexpr (R::LPR == 32) {
+    if (steps <= a.wpr * HIGH) norm_launch<T, R, HIGH, FP8>(a, warps, s);
+    else norm_launch<T, R, 0, FP8>(a, warps, s);
+  }
 }
 template <bool FP8> static void norm_types(const NormArgs &a, int dtype, bool vec, int sms, cudaStream_t s) {
-  if (dtype == GPHL_F32) vec ? norm_dispatch<float, false, FP8>(a, sms, s) : norm_dispatch<float, true, FP8>(a, sms, s);
-  else if (dtype == GPHL_BF16) vec ? norm_dispatch<__nv_bfloat16, false, FP8>(a, sms, s) : norm_dispatch<__nv_bfloat16, true, FP8>(a, sms, s);
-  else vec ? norm_dispatch<__half, false, FP8>(a, sms, s) : norm_dispatch<__half, true, FP8>(a, sms, s);
+  if (dtype == GPHL_F32) with_lanes<float>(a.n, vec, [&](auto r) { norm_dispatch<float, decltype(r), FP8>(a, sms, s); });
+  else if (dtype == GPHL_BF16) with_lanes<__nv_bfloat16>(a.n, vec, [&](auto r) { norm_dispatch<__nv_bfloat16, decltype(r), FP8>(a, sms, s); });
+  else with_lanes<__half>(a.n, vec, [&](auto r) { norm_dispatch<__half, decltype(r), FP8>(a, sms, s); });
 }
 
 static int sm_count() {
@@ -359,37 +350,33 @@ static int sm_count() {
 }
 
 struct GradShape {
-  int wpr, warps, grid, nv;
+  int wpr, warps, grid;
   size_t smem;
 };
-// E: values of a lane's step.  At most 16 values a lane are held (registers: two row operands and the gathering dw); nv == 0: wider.
-static GradShape grad_shape(int64_t m, int n, int e, int sms) {
-  const int steps = (n + 32 * e - 1) / (32 * e), hold = 16 / e;
+// E, LPR as in Row.  wpr == 0: wider than 32 warps hold.
+static GradShape grad_shape(int64_t m, int n, int e, int lpr, int sms) {
+  const int steps = (n + lpr * e - 1) / (lpr * e), hold = 8 / e;
   GradShape g{};
-  g.wpr = pow2_at_least((steps + hold - 1) / hold);
-  if (g.wpr > 16) {
-    g.wpr = 16, g.warps = 16, g.nv = 0;
+  const int wpr = pow2_at_least((steps + hold - 1) / hold);
+  if (wpr > 32) {
     g.grid = (int)std::min<int64_t>(m, 64);          // row groups of the separate dw kernel
     return g;
   }
-  g.nv = steps <= g.wpr * (hold / 2) ? hold / 2 : hold;
-  g.warps = g.wpr == 1 ? 8 : g.wpr;
-  const int per_block = g.warps / g.wpr;
-  // 32 warps an SM: the partial rows of dw stay few
-  g.grid = (int)std::min<int64_t>((m + per_block - 1) / per_block, (int64_t)sms * (32 / g.warps));
-  g.smem = g.wpr == 1 ? (size_t)g.warps * n * sizeof(float) : 0;
+  g.wpr = wpr, g.warps = wpr > 1 ? wpr : 8;
+  const int slots = g.warps / g.wpr * (32 / lpr);
+  g.grid = (int)std::min<int64_t>((m + slots - 1) / slots, (int64_t)sms * (32 / g.warps));
+  g.smem = g.wpr == 1 ? (size_t)slots * n * sizeof(float) : 0;
   return g;
 }
-template <typename T, bool SC> static void grad_launch(NormGradArgs a, const GradShape &g, cudaStream_t s) {
-  constexpr int HOLD = 16 / Row<T, SC>::E;
+template <typename T, typename R> static void grad_launch(NormGradArgs a, int sms, GradShape &g, cudaStream_t s) {
+  g = grad_shape(a.m, a.n, R::E, R::LPR, sms);
   a.wpr = g.wpr;
-  if (g.nv == 0) {
-    rms_norm_grad_wide_kernel<T, SC><<<(unsigned)a.m, 512, 0, s>>>(a);
+  if (g.wpr > 0) {
+    rms_norm_grad_kernel<T, R><<<g.grid, g.warps * 32, g.smem, s>>>(a);
+  } else if constexpr (R::LPR == 32) {
+    a.wpr = 16;
+    rms_norm_grad_wide_kernel<T, R><<<(unsigned)a.m, 512, 0, s>>>(a);
     rms_norm_dw_wide_kernel<T><<<dim3((unsigned)((a.n + 255) / 256), (unsigned)g.grid), 256, 0, s>>>(a);
-  } else if (g.nv == HOLD) {
-    rms_norm_grad_kernel<T, SC, HOLD><<<g.grid, g.warps * 32, g.smem, s>>>(a);
-  } else {
-    rms_norm_grad_kernel<T, SC, HOLD / 2><<<g.grid, g.warps * 32, g.smem, s>>>(a);
   }
 }
 
@@ -441,9 +428,10 @@ extern "C" int gphl_rms_norm_fp8(int32_t dtype, int64_t m, int64_t n, const void
 
 extern "C" int64_t gphl_rms_norm_grad_workspace_bytes(int32_t dtype, int64_t m, int64_t n) {
   if (m <= 0 || n <= 0 || dtype < GPHL_F32 || dtype > GPHL_F16) return 0;
-  // the vector or the column form may run (alignment is known at the call): the larger of the two
+  // any form may run (alignment is known at the call): the largest
   const int sms = sm_count();
-  const int64_t grid = std::max(grad_shape(m, (int)n, 4, sms).grid, grad_shape(m, (int)n, 16 / elem_size(dtype), sms).grid);
+  int64_t grid = grad_shape(m, (int)n, 4, 32, sms).grid;
+  for (int lpr = 8; lpr <= 32; lpr *= 2) grid = std::max<int64_t>(grid, grad_shape(m, (int)n, 16 / elem_size(dtype), lpr, sms).grid);
   return grid * n * (int64_t)sizeof(float);
 }
 
@@ -465,16 +453,17 @@ extern "C" int gphl_rms_norm_grad(int32_t dtype, int64_t m, int64_t n, const voi
   a.r = r, a.w = w, a.rstd = rstd, a.dy = dy, a.dr = dr, a.dx = dx, a.part = static_cast<float *>(workspace);
   a.m = m, a.n = (int32_t)n, a.w_f32 = w_dtype == GPHL_F32;
   const bool vec = norm_vec(n, dtype, {r, w, dy, dr, dx});
-  const GradShape g = grad_shape(m, (int)n, vec ? 16 / elem_size(dtype) : 4, sm_count());
-  if (dtype == GPHL_F32) vec ? grad_launch<float, false>(a, g, stream) : grad_launch<float, true>(a, g, stream);
-  else if (dtype == GPHL_BF16) vec ? grad_launch<__nv_bfloat16, false>(a, g, stream) : grad_launch<__nv_bfloat16, true>(a, g, stream);
-  else vec ? grad_launch<__half, false>(a, g, stream) : grad_launch<__half, true>(a, g, stream);
+  GradShape g{};
+  const int sms = sm_count();
+  if (dtype == GPHL_F32) with_lanes<float>(n, vec, [&](auto k) { grad_launch<float, decltype(k)>(a, sms, g, stream); });
+  else if (dtype == GPHL_BF16) with_lanes<__nv_bfloat16>(n, vec, [&](auto k) { grad_launch<__nv_bfloat16, decltype(k)>(a, sms, g, stream); });
+  else with_lanes<__half>(n, vec, [&](auto k) { grad_launch<__half, decltype(k)>(a, sms, g, stream); });
   int rc = launched("rms_norm_grad_kernel");
   if (rc != GPHL_OK) return rc;
   const unsigned blocks = (unsigned)((n + 31) / 32);
-  if (w_dtype == GPHL_F32) rms_norm_dw_kernel<float><<<blocks, 256, 0, stream>>>(a.part, g.grid, (int32_t)n, static_cast<float *>(dw));
+  if (w_dtype == GPHL_F32) rms_norm_dw_kernel<float><<<blocks, 1024, 0, stream>>>(a.part, g.grid, (int32_t)n, static_cast<float *>(dw));
   else if (w_dtype == GPHL_BF16)
-    rms_norm_dw_kernel<__nv_bfloat16><<<blocks, 256, 0, stream>>>(a.part, g.grid, (int32_t)n, static_cast<__nv_bfloat16 *>(dw));
-  else rms_norm_dw_kernel<__half><<<blocks, 256, 0, stream>>>(a.part, g.grid, (int32_t)n, static_cast<__half *>(dw));
+    rms_norm_dw_kernel<__nv_bfloat16><<<blocks, 1024, 0, stream>>>(a.part, g.grid, (int32_t)n, static_cast<__nv_bfloat16 *>(dw));
+  else rms_norm_dw_kernel<__half><<<blocks, 1024, 0, stream>>>(a.part, g.grid, (int32_t)n, static_cast<__half *>(dw));
   return launched("rms_norm_dw_kernel");
 }

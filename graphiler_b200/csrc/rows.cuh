@@ -1,11 +1,13 @@
-// Row access shared by the row-wise dense kernels (norm.cu, fp8.cu): a warp walks a row in steps, every lane holding E values of
-// a step as floats.  Aligned rows: E values of one 16-byte vector (a step is 128 fp32 or 256 16-bit columns).  Rows of odd width
-// or base: four single columns 32 apart (a step is 128 columns), so that a step's loads are still whole 128- or 64-byte lines.
+// Row access shared by the row-wise dense kernels (norm.cu, fp8.cu): LPR lanes walk a row in steps, every lane holding E values of
+// a step.  Aligned rows: E values of one 16-byte vector; rows narrower than a warp's 32 vectors share a warp (LPR = 8 or 16).  Rows of odd
+// width or base (SC): four single columns 32 apart, so that a step's loads are still whole 128- or 64-byte lines.
 #pragma once
 
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <float.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -21,11 +23,47 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-template <typename T, bool SC> struct Row {
-  static constexpr int E = SC ? 4 : 16 / (int)sizeof(T);
-  static constexpr int STEP = 32 * E;
+template <typename T, bool SC, int LPR_ = 32> struct Row {
+  static_assert(!SC || LPR_ == 32, "single columns are dealt to whole warps");
+  static constexpr bool SINGLE = SC;
+  static constexpr int LPR = LPR_, E = SC ? 4 : 16 / (int)sizeof(T), STEP = LPR * E;
+  struct Raw {                                        // a lane's values of a step: four words as stored, or four single values widened
+    uint32_t w[4];
+  };
+  // `lane`: of the row's LPR lanes
   __device__ static __forceinline__ int col(int step, int lane, int j) {
     return SC ? step * STEP + lane + 32 * j : step * STEP + lane * E + j;
+  }
+  __device__ static __forceinline__ Raw raw(const T *__restrict__ row, int step, int lane, int n) {
+    Raw x;
+    if constexpr (SC) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int c = col(step, lane, j);
+        x.w[j] = c < n ? __float_as_uint(to_float(row[c])) : 0u;
+      }
+    } else {
+      const int c = col(step, lane, 0);
+      const uint4 v = c < n ? *reinterpret_cast<const uint4 *>(row + c) : make_uint4(0, 0, 0, 0);
+      x.w[0] = v.x, x.w[1] = v.y, x.w[2] = v.z, x.w[3] = v.w;
+    }
+    return x;
+  }
+  __device__ static __forceinline__ void widen(const Raw &x, float (&v)[E]) {
+    if constexpr (E == 4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(x.w[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          v[2 * j] = __uint_as_float(x.w[j] << 16), v[2 * j + 1] = __uint_as_float(x.w[j] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x.w[j]));
+          v[2 * j] = f.x, v[2 * j + 1] = f.y;
+        }
+      }
+    }
   }
   // U: the stored type, T or float (a weight kept in 32 bits beside 16-bit rows)
   template <typename U> __device__ static __forceinline__ void load(const U *__restrict__ row, int step, int lane, int n, float (&v)[E]) {
@@ -36,7 +74,7 @@ template <typename T, bool SC> struct Row {
         v[j] = c < n ? to_float(row[c]) : 0.f;
       }
     } else {
-      constexpr int PER = 16 / (int)sizeof(U);      // values of one 16-byte load
+      constexpr int PER = 16 / (int)sizeof(U);        // values of one 16-byte load
       const int c = col(step, lane, 0);
       if (c < n) {
 #pragma unroll
@@ -74,6 +112,8 @@ template <typename T, bool SC> struct Row {
 
 // ---- e4m3 with a power-of-two scale per block of 128 -------------------------------------------------------------------------
 
+constexpr uint32_t ABS_BITS = 0x7fffffffu, INF_BITS = 0x7f800000u;
+
 // The exponent e >= -126 of the smallest power of two with amax <= 448 * 2^e (448 = 1.75 * 2^8, the largest e4m3 value).
 __device__ __forceinline__ int fp8_exponent(float amax) {
   const uint32_t b = __float_as_uint(amax);
@@ -88,45 +128,74 @@ __device__ __forceinline__ float finite_abs(float v) {
   const float a = fabsf(v);
   return a <= FLT_MAX ? a : 0.f;
 }
-__device__ __forceinline__ uint32_t e4m3(float v) {  // round to nearest even; infinities and NaN to the NaN code
-  const float t = fabsf(v) <= FLT_MAX ? v : __int_as_float(0x7fffffff);
-  return (uint32_t)__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3);
+// Two codes, round to nearest even; NaN to the NaN code.  `e4m3x2`: infinities too.
+__device__ __forceinline__ uint32_t e4m3x2_finite(float lo, float hi) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   lo = fabsf(lo) <= FLT_MAX ? lo : __int_as_float(0x7fffffff);
   hi = fabsf(hi) <= FLT_MAX ? hi : __int_as_float(0x7fffffff);
-  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+  return e4m3x2_finite(lo, hi);
 }
 
-// E bytes of codes of a lane's step; columns in [n, n_pad) are written as zero (the row's padding to 16 bytes).
-template <typename T, bool SC>
-__device__ __forceinline__ void store_codes(uint8_t *__restrict__ row, int step, int lane, int n, int n_pad, const uint32_t (&q)[Row<T, SC>::E]) {
-  using R = Row<T, SC>;
-  if constexpr (SC) {
+// The codes of a lane's values of one step, stored, and their block's scale.  All lanes of the warp call it; nothing is stored unless `live`.
+// Columns in [n, n_pad) are written as zero (the row's padding to 16 bytes).
+template <typename R>
+__device__ __forceinline__ void store_codes(const float (&y)[R::E], uint8_t *__restrict__ row, float *__restrict__ scale, int64_t scale_stride, int step, int lane,
+                                            int n, int n_pad, bool live) {
+  constexpr int E = R::E, BLOCK_LANES = R::STEP < 128 ? R::LPR : 128 / E;      // lanes that share a block
+  uint32_t big = 0;                                    // magnitudes compare as integers, and anything from infinity up is not finite
 #pragma unroll
-    for (int j = 0; j < R::E; ++j) {
+  for (int j = 0; j < E; ++j) big = max(big, __float_as_uint(y[j]) & ABS_BITS);
+#pragma unroll
+  for (int d = BLOCK_LANES / 2; d >= 1; d >>= 1) big = max(big, __shfl_xor_sync(FULL, big, d));
+  const bool rare = __any_sync(FULL, big >= INF_BITS);
+  if (rare) {                                          // the largest finite magnitude instead
+    float a = 0.f;
+#pragma unroll
+    for (int j = 0; j < E; ++j) a = fmaxf(a, finite_abs(y[j]));
+#pragma unroll
+    for (int d = BLOCK_LANES / 2; d >= 1; d >>= 1) a = fmaxf(a, __shfl_xor_sync(FULL, a, d));
+    big = __float_as_uint(a);
+  }
+  const int e = fp8_exponent(__uint_as_float(big));
+  const float inv = pow2f(-e);
+  uint32_t w[E / 4];
+  if (rare) {
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) w[i] = e4m3x2(y[4 * i] * inv, y[4 * i + 1] * inv) | (e4m3x2(y[4 * i + 2] * inv, y[4 * i + 3] * inv) << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i)
+      w[i] = e4m3x2_finite(y[4 * i] * inv, y[4 * i + 1] * inv) | (e4m3x2_finite(y[4 * i + 2] * inv, y[4 * i + 3] * inv) << 16);
+  }
+  const int c0 = R::col(step, lane, 0);
+  if (!live) return;
+  if constexpr (R::SINGLE) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
       const int c = R::col(step, lane, j);
-      if (c < n_pad) row[c] = c < n ? (uint8_t)q[j] : (uint8_t)0;
+      if (c < n_pad) row[c] = c < n ? (uint8_t)(w[0] >> (8 * j)) : (uint8_t)0;
     }
   } else {
-    const int c = R::col(step, lane, 0);
-    if (c < n_pad) {
-      uint32_t w[R::E / 4];
+    if (c0 < n_pad) {
 #pragma unroll
-      for (int i = 0; i < R::E / 4; ++i)
-        w[i] = c < n ? (q[4 * i] | (q[4 * i + 1] << 8) | (q[4 * i + 2] << 16) | (q[4 * i + 3] << 24)) : 0u;
-      if constexpr (R::E == 8) *reinterpret_cast<uint2 *>(row + c) = make_uint2(w[0], w[1]);
-      else *reinterpret_cast<uint32_t *>(row + c) = w[0];
+      for (int i = 0; i < E / 4; ++i) w[i] = c0 < n ? w[i] : 0u;
+      if constexpr (E == 8) *reinterpret_cast<uint2 *>(row + c0) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t *>(row + c0) = w[0];
     }
   }
+  const int block = c0 / 128;
+  if (lane % BLOCK_LANES == 0 && block * 128 < n) scale[block * scale_stride] = pow2f(e);
 }
 
-// Largest of the 128-column block that this lane's values belong to (16 lanes hold a block of a 16-bit vector step, else the warp).
-template <typename T, bool SC> __device__ __forceinline__ float block_max(float a) {
-  constexpr int LANES = 128 / Row<T, SC>::E;
-#pragma unroll
-  for (int d = LANES / 2; d >= 1; d >>= 1) a = fmaxf(a, __shfl_xor_sync(FULL, a, d));
-  return a;
+// Calls f with the number of lanes of a row as a constant: aligned rows of at most 8 or 16 vectors share a warp.
+template <typename T, typename F> static void with_lanes(int64_t n, bool vec, F f) {
+  const int64_t vectors = n * (int64_t)sizeof(T) / 16;
+  if (vec && vectors <= 8) f(Row<T, false, 8>());
+  else if (vec && vectors <= 16) f(Row<T, false, 16>());
+  else if (vec) f(Row<T, false, 32>());
+  else f(Row<T, true, 32>());
 }
 
 #endif  // __CUDACC__

@@ -306,7 +306,7 @@ int gphl_debug_reset_wait_timeouts(void); /* sets the counter back to 0 (synchro
  * kept for the backward pass.  y may be x, r may be x or residual. */
 int gphl_rms_norm(int32_t dtype, int64_t m, int64_t n, const void *x, const void *residual, const void *w, int32_t w_dtype, float eps,
                   void *y, void *r, float *rstd, void *stream);
-/* The same with y as codes: correctly rounded from the normalised value. */
+/* The same with y as codes (rounded once, from the fp32 value). */
 int gphl_rms_norm_fp8(int32_t dtype, int64_t m, int64_t n, const void *x, const void *residual, const void *w, int32_t w_dtype, float eps,
                       void *q, int64_t q_stride, float *scales, int64_t scale_stride, void *r, void *stream);
 /* dx = dr + rstd (g - xhat mean(g xhat)) with g = dy w, xhat = r rstd (dr may be NULL); dw = sum of dy xhat over the rows, in w's type,

@@ -22,7 +22,7 @@ def randn(*shape, seed=0, scale=1.0, dtype=F32):
 # ---- norm -----------------------------------------------------------------------------------------------------------
 
 NORM_SHAPES = [(1, 1), (1, 8), (3, 7), (5, 64), (2, 128), (257, 129), (33, 256), (1, 1000), (600, 1001), (64, 1024), (1, 4096), (9, 5000), (3, 8192),
-               (2, 12345), (2, 16400), (2, 40000)]
+               (2, 12345), (2, 16400), (2, 40000), (77, 16), (33, 40), (1000, 56), (9, 120)]
 
 
 @pytest.mark.parametrize("m,n", NORM_SHAPES)
@@ -111,7 +111,7 @@ def special_rows(m, n, dtype):
     return x
 
 
-@pytest.mark.parametrize("m,n", [(1, 1), (2, 16), (3, 127), (4, 128), (5, 129), (7, 1000), (130, 2050), (64, 4096)])
+@pytest.mark.parametrize("m,n", [(1, 1), (2, 16), (77, 24), (31, 64), (18, 104), (3, 127), (4, 128), (5, 129), (7, 1000), (130, 2050), (64, 4096)])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_quantize_and_dequantize(m, n, dtype):
     x = special_rows(m, n, dtype)
