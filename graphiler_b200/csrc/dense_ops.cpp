@@ -118,9 +118,11 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     const Tensor rows = rows_of(x);
     auto [y, r, rstd] = norm_run(rows, w, eps, res.defined() ? rows_of(res) : res, true);
     ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->save_for_backward({r.defined() ? r : rows, w, rstd});
+    // kept as the caller's own tensors, so that a change in place before the backward pass is noticed
+    if (r.defined()) r = r.view(x.sizes());
+    ctx->save_for_backward({r.defined() ? r : x.is_contiguous() ? x : rows, w, rstd});
     variable_list out{y.view(x.sizes())};
-    if (r.defined()) out.push_back(r.view(x.sizes()));
+    if (r.defined()) out.push_back(r);
     return out;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -128,7 +130,7 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
     const Tensor dy = grads[0], dr = grads.size() > 1 ? grads[1] : Tensor();
     if (!dy.defined()) return {dr, Tensor(), Tensor(), dr};         // only the sum went on: its gradient passes through
     const auto saved = ctx->get_saved_variables();
-    auto [dx, dw] = rms_norm_grad(saved[0], saved[1], saved[2], rows_of(dy), dr.defined() ? OptTensor(rows_of(dr)) : c10::nullopt);
+    auto [dx, dw] = rms_norm_grad(rows_of(saved[0]), saved[1], saved[2], rows_of(dy), dr.defined() ? OptTensor(rows_of(dr)) : c10::nullopt);
     dx = dx.view(ctx->saved_data["shape"].toIntVector());
     return {dx, dw, Tensor(), grads.size() > 1 ? dx : Tensor()};    // two outputs: there was a residual
   }
@@ -368,7 +370,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     auto [h, g, u] = gated_run(rows, wg, wu, act, rows.size(1) > RECOMPUTE_K);
     ctx->saved_data["shape"] = x.sizes().vec();
     ctx->saved_data["act"] = act;
-    ctx->save_for_backward({rows, wg, wu, g, u});
+    ctx->save_for_backward({x.is_contiguous() ? x : rows, wg, wu, g, u});
     auto shape = x.sizes().vec();
     shape.back() = wg.size(1);
     return h.view(shape);
@@ -377,7 +379,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     TORCH_CHECK(!at::GradMode::is_enabled(), "gated_linear: first derivatives only (create_graph is not supported)");
     const auto s = ctx->get_saved_variables();
     const bool need_x = ctx->needs_input_grad(0), need_g = ctx->needs_input_grad(1), need_u = ctx->needs_input_grad(2);
-    auto [dx, dg, du] = gated_grad_run(rows_of(grads[0]), s[3], s[4], s[0], s[1], s[2], ctx->saved_data["act"].toStringRef(), need_x, need_g || need_u);
+    auto [dx, dg, du] = gated_grad_run(rows_of(grads[0]), s[3], s[4], rows_of(s[0]), s[1], s[2], ctx->saved_data["act"].toStringRef(), need_x, need_g || need_u);
     return {need_x ? dx.view(ctx->saved_data["shape"].toIntVector()) : Tensor(), need_g ? dg : Tensor(), need_u ? du : Tensor(), Tensor()};
   }
 };

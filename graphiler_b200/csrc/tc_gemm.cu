@@ -33,7 +33,7 @@ struct __align__(64) GemmArgs {
   int64_t m, n;
   uint32_t tiles_m, tiles_n, work;                     // work = tiles_m * tiles_n * batch * splits < 2^31
   int32_t batch, splits, kt, kt_first;                 // steps of 128 bytes of k; kt_first: steps of the first pair (CONCAT)
-  int32_t a_mn, b_mn, types, stages;
+  int32_t a_mn, b_mn, types, a_bytes;                  // a_bytes: of one step's box of A (fewer rows than a tile where m is smaller)
   uint32_t idesc;
   const int32_t *ptr;
   void *out[2];
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS, FP8), 1) gemm_kernel(c
           const uint32_t s = i % STAGES, bar = lead_full + 8 * s, sa = ring_u + s * STAGE, sb = sa + GM * 128;
           if (!(ok = __all_sync(FULL, tc::mbar_wait(empty + 8 * s, ((i / STAGES) & 1) ^ 1, failed)))) break;
           if (tc::elect()) {
-            if (rank == 0) tc::mbar_expect_tx(full + 8 * s, CTAS * STAGE);
+            if (rank == 0) tc::mbar_expect_tx(full + 8 * s, CTAS * (a.a_bytes + BROWS * 128));
             const int sel = a.batch > 1 ? t.batch : (kt >= a.kt_first), x = (a.batch == 1 && kt >= a.kt_first ? kt - a.kt_first : kt) * KE;
             if (a.a_mn) {
 #pragma unroll
@@ -866,39 +866,47 @@ struct Shape {
   int64_t tiles_m, tiles_n;
   int32_t kt, batch;
 };
-// The widest tile that leaves no half of it empty (narrower tiles read A once more per column tile) and, parts of 8 steps counted,
-// still gives every SM something; then k split so that the work items fill the SMs: as many parts as make ceil(items / SMs) / items smallest, each of at least 4 steps, fewest parts first.
+// Tile width, blocks per tile and parts of k by an estimate of the time, in microseconds: waves of tiles times steps times the measured
+// time of a step (128 bytes of k: 0.40 for a pair of blocks with 256 columns in 16 bits, 0.50 for one block or in e4m3, less for narrower
+// tiles, which read A more often), at least the time of the operands' bytes at the rate that tiles of that width were seen to stream them, and
+// for parts their join (3, and the parts' fp32 sums written and read at 5 TB/s).  In e4m3: 2048 x 11264 -> 4096 takes 112 with k whole, 141 in
+// 2 parts; 1 x 4096 -> 8192 18.7 in 2 parts, 14.0 in 4; 1 x 16384 -> 16384 73 with 128 columns a tile, 59 with 256 and 2 parts.
 static bool paired(const GemmCall &c) { return c.dual == DUAL_GATED || c.dual == DUAL_GATED_GRAD; }
 static Shape shape_of(const GemmCall &c) {
-  Shape s{};
   const int ke = c.fp8 ? 128 : 64;
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  s.batch = c.dual == DUAL_BATCH ? 2 : 1;
-  const int64_t per = (c.k + ke - 1) / ke;
-  s.kt = (int32_t)(c.dual == DUAL_CONCAT ? 2 * per : per);
-  s.tiles_m = (c.m + GM - 1) / GM + (c.ptr ? std::min<int64_t>(c.types, c.m) : 0);
-  const int64_t wide = paired(c) ? 2 * c.n : c.n;
-  s.bn = wide > 128 ? 256 : (wide > 64 || paired(c)) ? 128 : 64;
-  if (c.q) s.bn = 256;                                   // a tile is one block of 128 codes
-  auto tiles = [&](int bn) { return s.tiles_m * ((wide + bn - 1) / bn) * s.batch; };
-  if (s.bn == 256 && !c.q && tiles(256) * std::max(1, s.kt / 8) < sms) s.bn = 128;
-  // pairs of blocks where the tiles of 256 rows are whole but for the last
-  s.ctas = s.bn == 256 && c.m > GM && (!c.ptr || c.m >= 4 * GM * c.types) ? 2 : 1;
-  if (s.ctas == 2) s.tiles_m = (c.m + 2 * GM - 1) / (2 * GM) + (c.ptr ? std::min<int64_t>(c.types, c.m) : 0);
-  const int out = paired(c) ? s.bn / 2 : s.bn, units = sms / s.ctas;
-  s.tiles_n = (c.n + out - 1) / out;
-  s.splits = 1;
-  const int64_t items = s.tiles_m * s.tiles_n * s.batch;
-  if (items < 2 * units) {
-    double best = 1e30;
-    for (int p = 1; p <= 64 && p * 4 <= s.kt; ++p) {
-      const double waves = (double)((items * p + units - 1) / units) / p;  // time in units of one unsplit tile
-      const double cost = waves * s.kt + 6.0 * (p > 1) + 0.15 * p;          // the join costs about six steps and grows with the parts
-      if (cost < best - 1e-9) best = cost, s.splits = p;
+  const bool two = paired(c);
+  const int64_t per = (c.k + ke - 1) / ke, wide = two ? 2 * c.n : c.n;
+  const double size = c.fp8 ? 1.0 : 2.0, pairs = c.dual == DUAL_NONE ? 1.0 : 2.0;
+  const double bytes = (((c.dual == DUAL_CONCAT || (c.dual == DUAL_BATCH && c.m != c.n) ? 2.0 : 1.0) * c.m * c.k + pairs * c.types * c.n * c.k) * size);
+  Shape best{};
+  double best_us = 1e30;
+  for (int bn = 256; bn >= 64; bn /= 2) {
+    if (two && bn == 64) continue;
+    if (c.q && bn != 256) continue;                      // a tile is one block of 128 codes
+    if (bn > 64 && wide <= bn / 2 && !(two && bn == 128) && !c.q) continue;
+    for (int ctas = 1; ctas <= 2; ++ctas) {
+      // pairs of blocks where the tiles of 256 rows are whole but for the last
+      if (ctas == 2 && (bn != 256 || c.m <= GM || (c.ptr && c.m < 4 * GM * c.types))) continue;
+      Shape s{};
+      s.bn = bn, s.ctas = ctas, s.batch = c.dual == DUAL_BATCH ? 2 : 1;
+      s.kt = (int32_t)(c.dual == DUAL_CONCAT ? 2 * per : per);
+      s.tiles_m = (c.m + ctas * GM - 1) / (ctas * GM) + (c.ptr ? std::min<int64_t>(c.types, c.m) : 0);
+      const int out = two ? bn / 2 : bn, units = sms / ctas;
+      s.tiles_n = (c.n + out - 1) / out;
+      const int64_t items = s.tiles_m * s.tiles_n * s.batch;
+      const double rate = bn == 256 ? 5.2e6 : bn == 128 ? 4.0e6 : 3.2e6;      // bytes a microsecond
+      const double step = bn == 256 ? (c.fp8 || ctas == 1 ? 0.50 : 0.40) : bn == 128 ? 0.32 : 0.24;
+      for (int p = 1; p == 1 || (p <= 64 && p * 4 <= s.kt && items < 2 * units); ++p) {
+        const double waves = (double)((items * p + units - 1) / units);
+        double us = std::max(waves * ((double)s.kt / p * step + 1.5), bytes / rate);
+        if (p > 1) us += 3.0 + (double)p * s.batch * c.m * wide * 8.0 / 5e6;
+        if (us < best_us * 0.999) best_us = us, best = s, best.splits = p;
+      }
     }
   }
-  return s;
+  return best;
 }
 static int64_t part_ld(const GemmCall &c) { return (c.n + 3) / 4 * 4 * (paired(c) ? 2 : 1); }
 
@@ -939,9 +947,13 @@ int gemm(const GemmCall &c, const char *what, cudaStream_t stream) {
   const bool pairs_of_b = paired(c);
   GemmArgs a{};
   const int pairs = c.dual == DUAL_NONE ? 1 : 2;
+  // With fewer rows than a tile, only they are brought: the tensor core multiplies whatever the stage's other rows hold into rows of the
+  // accumulator that nobody reads.  (A box of 128 rows costs its time even where it is zeros: 5 x 4096 -> 11264 47 us.)
+  const int a_rows = c.a_mn ? 64 : (int)std::min<int64_t>(GM, (c.m + 7) / 8 * 8);
+  a.a_bytes = c.a_mn ? GM * 128 : a_rows * 128;
   for (int i = 0; i < pairs; ++i) {
     if (i == 0 || !pairs_of_b) {
-      int rc = encode(&a.a[i], c.a[i], c.in_type, c.fp8, c.a_mn ? 64 : GM, what);
+      int rc = encode(&a.a[i], c.a[i], c.in_type, c.fp8, a_rows, what);
       if (rc != GPHL_OK) return rc;
     }
     int rc = encode(&a.b[i], c.b[i], c.in_type, c.fp8, c.b_mn ? 64 : pairs_of_b ? s.bn / 2 : s.bn / s.ctas, what);

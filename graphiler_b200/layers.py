@@ -17,7 +17,7 @@ from typing import Dict, Optional
 
 import torch
 
-from . import capi
+from . import capi, dense
 from .graph import GraphArrays
 
 
@@ -161,3 +161,27 @@ def hgt_layer(pg: PreparedGraph, h, p: Dict[str, torch.Tensor], heads: int, sqrt
     out = capi.segment_mm(t, p["a_weight"], g.ntype_pointer)
     alpha = capi.gather_rows(g.ntype_COO, torch.sigmoid(p["skip"]).unsqueeze(1).contiguous())
     return out.mul_(alpha)
+
+
+def feed_forward_layer(h, p: Dict[str, torch.Tensor], residual=None, eps: float = 1e-6, activation: str = "silu"):
+    """Pre-norm gated feed-forward of a graph transformer on the node rows, after its attention layer (``hgt_layer``): with r = h (+
+    ``residual``, e.g. the attention's input), returns ``r + (act(n Wg) * (n Wu)) Wd`` for ``n = rms_norm(r)``.  bfloat16 or float16 rows,
+    differentiable: norm and gated product are one autograd node each; the product back is plain cuBLAS, as the other dense projections.
+    ``p``: norm_weight (d), gate_weight and up_weight (d, f), down_weight (f, d)."""
+    n = dense.rms_norm(h, p["norm_weight"], eps, residual=residual)
+    n, r = (n, h) if residual is None else n
+    return r + torch.matmul(dense.gated_linear(n, p["gate_weight"], p["up_weight"], activation), p["down_weight"])
+
+
+def prepare_feed_forward_fp8(p: Dict[str, torch.Tensor]):
+    """The weights of ``feed_forward_layer`` in 8 bits, laid out once for ``feed_forward_layer_fp8``."""
+    return {"norm_weight": p["norm_weight"], **{k: capi.quantize_fp8_weight(p[k].contiguous()) for k in ("gate_weight", "up_weight", "down_weight")}}
+
+
+def feed_forward_layer_fp8(h, q, residual=None, eps: float = 1e-6, activation: str = "silu"):
+    """``feed_forward_layer`` for serving, in 8 bits: three kernels, the rows between them e4m3 with a scale per 128 values; the sum
+    with r is in the rows' type.  ``q``: ``prepare_feed_forward_fp8``."""
+    n = capi.rms_norm_fp8(h, q["norm_weight"], eps, residual=residual)
+    n, r = (n, h) if residual is None else n
+    g = capi.gated_linear_fp8(n, q["gate_weight"], q["up_weight"], activation)
+    return capi.segment_mm_fp8(g, q["down_weight"], out_dtype=h.dtype).add_(r)

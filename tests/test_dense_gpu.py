@@ -361,3 +361,165 @@ def test_gated_gradient_against_differences():
         num = (f(h) - f(-h)) / (2 * h)
         bound = float(((err + ref.half_step(F16) * a.double().abs() + 2.0 ** -25) * d.abs()).sum()) + 1e-5 * float((a.double().abs() * d.abs()).sum())
         assert abs(float(num - (a.double() * d).sum())) <= bound
+
+
+# ---- the operators together -------------------------------------------------------------------------------------------
+
+def ff_inputs(n, d, f, dtype):
+    p = {"norm_weight": 1 + 0.2 * randn(d, seed=7), "gate_weight": randn(d, f, seed=8, scale=d ** -0.5), "up_weight": randn(d, f, seed=9, scale=d ** -0.5),
+         "down_weight": randn(f, d, seed=10, scale=f ** -0.5)}
+    return randn(n, d, seed=11, dtype=dtype), randn(n, d, seed=12, dtype=dtype), {k: v.to(dtype) for k, v in p.items()}
+
+
+def ff_ref(h, res, p, rows=lambda v: v, weight=lambda w: w.double()):
+    """The block in 64 bits; `rows` and `weight`: what is rounded on the way."""
+    r = h if res is None else (h.float() + res.float()).to(h.dtype)
+    y = rows(ref.rms_norm(r, None, p["norm_weight"], 1e-6)[2])
+    g, u = y @ weight(p["gate_weight"]), y @ weight(p["up_weight"])
+    return r.double() + rows(ref.act(g, "silu")[0] * u) @ weight(p["down_weight"])
+
+
+@pytest.mark.parametrize("n,d,f", [(1, 64, 128), (50, 96, 200), (300, 256, 640)])
+@pytest.mark.parametrize("with_res", [False, True])
+def test_feed_forward_layer(n, d, f, with_res):
+    from graphiler_b200 import layers
+    h, res, p = ff_inputs(n, d, f, BF16)
+    res = res if with_res else None
+    leaves = [t.requires_grad_(True) for t in (h, *p.values())] + ([res.requires_grad_(True)] if with_res else [])
+    out = layers.feed_forward_layer(h, p, residual=res)
+    want = ff_ref(h.detach(), None if res is None else res.detach(), {k: v.detach() for k, v in p.items()})
+    # every element of n, of the gated rows, of the product and of the sum is rounded once, half a step of bf16 each: relative to
+    # the values' own size, and the three products average what is random in it; four half steps of the largest value cover the sum
+    assert float((out.detach().double() - want).abs().max()) <= 4 * ref.half_step(BF16) * float(want.abs().max()) * 2
+    grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    # the same through 64-bit autograd
+    leaves64 = [t.detach().double().requires_grad_(True) for t in leaves]
+    h64, w64 = leaves64[0], dict(zip(p, leaves64[1:1 + len(p)]))
+    r = h64 + (leaves64[-1] if with_res else 0)
+    y = r * torch.rsqrt(r.square().mean(dim=1, keepdim=True) + 1e-6) * w64["norm_weight"]
+    o = r + (torch.nn.functional.silu(y @ w64["gate_weight"]) * (y @ w64["up_weight"])) @ w64["down_weight"]
+    for a, b in zip(grads, torch.autograd.grad(o, leaves64, torch.ones_like(o))):
+        # eight roundings of half a step on the longest way (sum, n, gated rows, their gradients, dx, the norm's gradient)
+        assert float((a.double() - b).norm()) <= 8 * ref.half_step(BF16) * float(b.norm())
+
+
+@pytest.mark.parametrize("n,d,f", [(1, 128, 256), (50, 200, 333), (700, 512, 1024)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_feed_forward_layer_fp8(n, d, f, dtype):
+    from graphiler_b200 import layers
+    h, res, p = ff_inputs(n, d, f, dtype)
+    q = layers.prepare_feed_forward_fp8(p)
+    got = layers.feed_forward_layer_fp8(h, q, residual=res)
+    want = ff_ref(h, res, p, rows=lambda v: ref.quantize_rows(v)[0], weight=lambda w: ref.quantize_weight(w[None])[0][0].t())
+    # codes next to a border may fall on its other side: a share of about 2^-20 / 2^-4 of them moves by 2^-3 in n, which moves g and u by
+    # 2^-3 sqrt(2^-16) = 2^-11 relative, so that a share of 2^-7 of the second codes moves by 2^-3: 2^-6.5 of the product; plus the output's rounding
+    r = (h.float() + res.float()).double()
+    assert float((got.double() - want).norm()) <= 2.0 ** -6.5 * float((want - r).norm()) + 2 * ref.half_step(dtype) * float(want.norm())
+
+
+# ---- two calls at once, captured calls, streams ---------------------------------------------------------------------------
+
+def test_two_streams_at_once():
+    c = capi()
+    x, w = codes(500, 2048, 1), weights(1, 2048, 640, 2)
+    a, b = randn(300, 512, seed=3, dtype=BF16), randn(512, 384, seed=4, dtype=BF16)
+    want = c.segment_mm_fp8(x, w), c.gated_linear(a, b, b)
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(5):
+        with torch.cuda.stream(s1):
+            got.append(c.segment_mm_fp8(x, w))
+        with torch.cuda.stream(s2):
+            got.append(c.gated_linear(a, b, b))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert torch.equal(g, want[i % 2])
+
+
+def test_captured_calls_keep_their_scratch_apart():
+    """Two graphs whose calls need scratch (k is split), replayed in turn and with new inputs."""
+    c = capi()
+    w = weights(1, 4096, 512, 2)
+    ws = [randn(2048, 256, seed=s, dtype=BF16) for s in (5, 6)]
+    xs = [codes(3, 4096, 1), codes(5, 4096, 7)]
+    rows = [randn(4, 2048, seed=8, dtype=BF16), randn(9, 2048, seed=9, dtype=BF16)]
+    def call(i):
+        y, r = c.rms_norm(rows[i], ws[0][:, 0].contiguous(), residual=rows[i])
+        return c.segment_mm_fp8(xs[i], w), c.gated_linear(y, *ws)
+    want = [call(0), call(1)]
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call(i))
+        graphs.append(g)
+    for _ in range(3):
+        for i in (0, 1, 1, 0):
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for o, v in zip(outs, want):
+            assert all(torch.equal(a, b) for a, b in zip(o, v))
+    rows[0].copy_(randn(4, 2048, seed=20, dtype=BF16))
+    graphs[0].replay()
+    assert torch.equal(outs[0][1], call(0)[1])
+    del graphs, outs
+
+
+def test_captured_training_step():
+    from graphiler_b200 import dense
+    x, wg, wu, dh = gated_inputs(40, 96, 128, BF16, False)
+    nw, leaves = torch.ones(96, device="cuda", dtype=BF16).requires_grad_(True), [t.requires_grad_(True) for t in (x, wg, wu)]
+    def step():
+        h = dense.gated_linear(dense.rms_norm(x, nw), wg, wu, "gelu")
+        return torch.autograd.grad(h, leaves + [nw], dh)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        want = step()
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    del g
+
+
+def test_results_repeat_bit_for_bit():
+    c = capi()
+    x, wg, wu, dh = gated_inputs(1500, 96, 264, BF16, False)
+    first = c.gated_linear_grad(dh, None, None, x, wg, wu)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, c.gated_linear_grad(dh, None, None, x, wg, wu)))
+    r, w, rstd = x, wg[:, 0].contiguous(), c.rms_norm(x, wg[:, 0].contiguous(), return_rstd=True)[1]
+    first = c.rms_norm_grad(r, w, rstd, x)
+    assert all(torch.equal(a, b) for a, b in zip(first, c.rms_norm_grad(r, w, rstd, x)))
+
+
+def test_no_wait_ran_out():
+    assert capi().tc_wait_timeouts() == 0
+
+
+# ---- empty inputs ------------------------------------------------------------------------------------------------------
+
+def test_empty_inputs():
+    c = capi()
+    e = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype, device="cuda")
+    assert c.rms_norm(e(0, 64), e(64)).shape == (0, 64) and c.rms_norm(e(3, 0), e(0)).shape == (3, 0)
+    dx, dw = c.rms_norm_grad(e(0, 64), e(64) + 1, e(0, dtype=F32), e(0, 64))
+    assert dx.shape == (0, 64) and (dw == 0).all()
+    q = c.quantize_fp8(e(0, 64))
+    assert q.values.shape == (0, 64) and c.dequantize_fp8(q).shape == (0, 64)
+    w = c.quantize_fp8_weight(e(64, 32))
+    assert c.segment_mm_fp8(q, w).shape == (0, 32)
+    assert c.segment_mm_fp8(c.quantize_fp8(e(5, 64)), c.quantize_fp8_weight(e(64, 0))).shape == (5, 0)
+    assert (c.segment_mm_fp8(c.quantize_fp8(e(5, 0)), c.quantize_fp8_weight(e(0, 32))) == 0).all()
+    assert (c.gated_linear(e(5, 0), e(0, 8), e(0, 8)) == 0).all() and c.gated_linear(e(0, 4), e(4, 8), e(4, 8)).shape == (0, 8)
+    dx, dg, du = c.gated_linear_grad(e(0, 8), None, None, e(0, 4), e(4, 8) + 1, e(4, 8))
+    assert dx.shape == (0, 4) and (dg == 0).all() and (du == 0).all()
+    h = c.gated_linear_fp8(c.quantize_fp8(e(0, 64)), w, w)
+    assert h.values.shape == (0, 32)
+    z = c.gated_linear_fp8(c.quantize_fp8(e(4, 64)), w, w)
+    assert (c.dequantize_fp8(z) == 0).all()
