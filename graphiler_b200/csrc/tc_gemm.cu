@@ -179,20 +179,6 @@ __device__ __forceinline__ void ld_wait(float (&f)[32]) {
                : "memory");
 }
 
-// The same for 16 columns.
-__device__ __forceinline__ void ld16(uint32_t taddr, float (&f)[16]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-               : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]), "=f"(f[8]), "=f"(f[9]), "=f"(f[10]), "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15])
-               : "r"(taddr)
-               : "memory");
-}
-__device__ __forceinline__ void ld_wait(float (&f)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+f"(f[0]), "+f"(f[1]), "+f"(f[2]), "+f"(f[3]), "+f"(f[4]), "+f"(f[5]), "+f"(f[6]), "+f"(f[7]), "+f"(f[8]), "+f"(f[9]), "+f"(f[10]), "+f"(f[11]), "+f"(f[12]), "+f"(f[13]), "+f"(f[14]), "+f"(f[15])
-               :
-               : "memory");
-}
-
 }  // namespace tc
 
 // ---- tiles -------------------------------------------------------------------------------------------------------------------------
@@ -423,10 +409,10 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS, FP8), 1) gemm_kernel(c
   tc::after_sync();
   const uint32_t tmem = s_tmem;
   const uint32_t w0 = blockIdx.x / CTAS, wstep = gridDim.x / CTAS;
-  // e4m3: 12 warps start with 168 registers a thread (64512 of them); the 8 that hold sums take 216 and the 4 others give theirs up
+  // e4m3: 12 warps start with 168 registers a thread (64512 of them); the 8 that hold sums take 232 and the 4 others give theirs up
   static_assert(!FP8 || EPI_WARPS == 8, "the register split is for 8 + 4 warps");
   if (warp >= EPI_WARPS) {
-    if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == EPI_WARPS) {
       // ---- TMA: step i goes to stage i % STAGES; the bytes of both blocks are counted on the even block's barrier
       uint32_t i = 0;
@@ -510,7 +496,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS, FP8), 1) gemm_kernel(c
       }
     }
   } else {
-    if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");
     // ---- epilogue: warp w reads lanes 32 (w % 4) .. and part w / 4 of the columns
     const int cpart = warp >> 2, quad = warp & 3;
     uint8_t *stg = ring + RING_BYTES + warp * STAGING;
@@ -614,13 +600,12 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS, FP8), 1) gemm_kernel(c
           ok = __all_sync(FULL, tc::mbar_wait(acc_full + 8 * (acc & 1), (acc >> 1) & 1, failed));
           tc::after_sync();
         };
-        // 16 columns (half a chunk) at a time, two of them in registers in turn: while one is scaled and added, the next is on its way
-        // from tensor memory, the first of the next accumulator included.
-        constexpr int HALVES = 2 * NCH;
-        auto addr = [&](int h) { return tmem + (acc & 1) * BN + ((uint32_t)(quad * 32) << 16) + acc_col(h / 2) + 16 * (h & 1); };
-        float v[2][16];
+        // Two chunks in registers in turn: while one is scaled and added, the next is on its way from tensor memory, the first of the next
+        // accumulator included.
+        auto addr = [&](int c) { return tmem + (acc & 1) * BN + ((uint32_t)(quad * 32) << 16) + acc_col(c); };
+        float v[2][32];
         ready();
-        if (ok) tc::ld16(addr(0), v[0]);
+        if (ok) tc::ld32(addr(0), v[0]);
         for (int kt = k0; kt < k1 && ok; ++kt) {
           if ((kt - k0) % SCALES == 0) {
             if (kt > k0) fetch(kt + SCALES);             // into the group that has just been used up (by this thread alone)
@@ -634,21 +619,27 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS, FP8), 1) gemm_kernel(c
             if (PAIRED) next_w1 = __ldg(sw1 + kt + 1);
           }
 #pragma unroll
-          for (int h = 0; h < HALVES; ++h) {
-            tc::ld_wait(v[h & 1]);
-            if (h + 1 < HALVES) {
-              tc::ld16(addr(h + 1), v[(h + 1) & 1]);
+          for (int c = 0; c < NCH; ++c) {
+            constexpr int LAST = NCH - 1;
+            float (&u)[32] = v[NCH == 1 ? 0 : c & 1];
+            tc::ld_wait(u);
+            if (c < LAST) {
+              tc::ld32(addr(c + 1), v[(c + 1) & 1]);
             } else {
               release();
               ++acc;
-              if (kt + 1 < k1) {
+              if (NCH > 1 && kt + 1 < k1) {
                 ready();
-                if (ok) tc::ld16(addr(0), v[0]);
+                if (ok) tc::ld32(addr(0), v[0]);
               }
             }
-            const uint64_t s = PAIRED && h >= NCH ? p1 : p0;
+            const uint64_t s = PAIRED && c >= NCH / 2 ? p1 : p0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum[h / 2][(h & 1) * 8 + i] = ffma2(pack2(v[h & 1][2 * i], v[h & 1][2 * i + 1]), s, sum[h / 2][(h & 1) * 8 + i]);
+            for (int i = 0; i < 16; ++i) sum[c][i] = ffma2(pack2(u[2 * i], u[2 * i + 1]), s, sum[c][i]);
+            if (NCH == 1 && kt + 1 < k1) {
+              ready();
+              if (ok) tc::ld32(addr(0), v[0]);
+            }
           }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -867,7 +858,7 @@ struct Shape {
   int32_t kt, batch;
 };
 // Tile width, blocks per tile and parts of k by an estimate of the time, in microseconds: waves of tiles times steps times the measured
-// time of a step (128 bytes of k: 0.40 for a pair of blocks with 256 columns in 16 bits, 0.50 for one block or in e4m3, less for narrower
+// time of a step (128 bytes of k: 0.40 for a pair of blocks with 256 columns in 16 bits, 0.48 in e4m3, 0.50 for one block, less for narrower
 // tiles, which read A more often), at least the time of the operands' bytes at the rate that tiles of that width were seen to stream them, and
 // for parts their join (3, and the parts' fp32 sums written and read at 5 TB/s).  In e4m3: 2048 x 11264 -> 4096 takes 112 with k whole, 141 in
 // 2 parts; 1 x 4096 -> 8192 18.7 in 2 parts, 14.0 in 4; 1 x 16384 -> 16384 73 with 128 columns a tile, 59 with 256 and 2 parts.
@@ -897,7 +888,7 @@ static Shape shape_of(const GemmCall &c) {
       s.tiles_n = (c.n + out - 1) / out;
       const int64_t items = s.tiles_m * s.tiles_n * s.batch;
       const double rate = bn == 256 ? 5.2e6 : bn == 128 ? 4.0e6 : 3.2e6;      // bytes a microsecond
-      const double step = bn == 256 ? (c.fp8 || ctas == 1 ? 0.50 : 0.40) : bn == 128 ? 0.32 : 0.24;
+      const double step = bn == 256 ? (ctas == 1 ? 0.50 : c.fp8 ? 0.48 : 0.40) : bn == 128 ? 0.32 : 0.24;
       for (int p = 1; p == 1 || (p <= 64 && p * 4 <= s.kt && items < 2 * units); ++p) {
         const double waves = (double)((items * p + units - 1) / units);
         double us = std::max(waves * ((double)s.kt / p * step + 1.5), bytes / rate);
