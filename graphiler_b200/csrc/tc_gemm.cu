@@ -28,10 +28,24 @@ constexpr int RASTER = 16;                             // row tiles that are wal
 
 __device__ int g_gemm_wait_timeouts = 0;
 
+// n / d for n < 2^31 by one multiplication: mul = ceil(2^(32 + shift) / d) with 2^shift < d <= 2^(shift + 1) (Granlund and Montgomery, Division by
+// Invariant Integers using Multiplication); d == 1 is its own case.
+struct Divisor {
+  uint32_t d, mul, shift;
+  __host__ void set(uint32_t v) {
+    d = v, mul = shift = 0;
+    if (v <= 1) return;
+    while ((2u << shift) < v) ++shift;
+    mul = (uint32_t)(((1ull << (32 + shift)) + v - 1) / v);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return d <= 1 ? n : __umulhi(n, mul) >> shift; }
+};
+
 struct __align__(64) GemmArgs {
   CUtensorMap a[2], b[2];
   int64_t m, n;
   uint32_t tiles_m, tiles_n, work;                     // work = tiles_m * tiles_n * batch * splits < 2^31
+  Divisor by_plane, by_band, by_last;                  // tiles of a plane, of a band of RASTER row tiles, row tiles of the last band
   int32_t batch, splits, kt, kt_first;                 // steps of 128 bytes of k; kt_first: steps of the first pair (CONCAT)
   int32_t a_mn, b_mn, types, a_bytes;                  // a_bytes: of one step's box of A (fewer rows than a tile where m is smaller)
   uint32_t idesc;
@@ -196,13 +210,14 @@ template <int CTAS> __device__ __forceinline__ Tile find_tile(const GemmArgs &a,
   const uint32_t plane = a.tiles_m * a.tiles_n;
   t.split = t.batch = 0;
   if (w >= plane) {
-    const uint32_t p = w / plane;
+    const uint32_t p = a.by_plane.div(w);
     w -= p * plane;
-    t.split = (int)(p / (uint32_t)a.batch), t.batch = (int)(p % (uint32_t)a.batch);
+    t.split = (int)(a.batch == 2 ? p >> 1 : p), t.batch = (int)(a.batch == 2 ? p & 1 : 0);
   }
-  const uint32_t band = w / (RASTER * a.tiles_n), in = w - band * RASTER * a.tiles_n;
-  const uint32_t high = min((uint32_t)RASTER, a.tiles_m - band * RASTER);
-  const uint32_t nt = in / high;
+  const uint32_t band = a.by_band.div(w), in = w - band * RASTER * a.tiles_n;
+  const bool whole = (band + 1) * RASTER <= a.tiles_m;
+  const uint32_t high = whole ? RASTER : a.tiles_m - band * RASTER;
+  const uint32_t nt = whole ? in / RASTER : a.by_last.div(in);
   const int64_t mt = band * RASTER + (in - nt * high);
   t.n0 = (int)nt * bn_out;
   t.seg = 0;
@@ -504,16 +519,19 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS, FP8), 1) gemm_kernel(c
     uint32_t acc = 0, tiles = 0;                         // accumulators read; tiles of codes finished
     bool ok = true;
     // GATED_GRAD: chunk c of work item w of dh, on its way into the upper half of the staging buffer
-    auto fetch_dh = [&](uint32_t w, int c) {
-      if (w < a.work) {
-        const Tile t = find_tile<CTAS>(a, w, BN_OUT, lane);
+    auto fetch_dh = [&](const Tile &t, int c) {
+      if (t.rows > 0) {
         fetch_chunk(a.dh, a.n, t.row0 + rank * GM + quad * 32, t.rows - rank * GM - quad * 32, (int64_t)t.n0 + cpart * (BN_OUT / PARTS) + 32 * c, a.n, stg + 2048, lane);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (MODE == GATED_GRAD && a.dh_vec && a.splits == 1) fetch_dh(w0, 0);
+    Tile next{};
+    if (w0 < a.work) next = find_tile<CTAS>(a, w0, BN_OUT, lane);
+    if (MODE == GATED_GRAD && a.dh_vec && a.splits == 1) fetch_dh(next, 0);
     for (uint32_t w = w0; w < a.work && ok; w += wstep) {
-      const Tile t = find_tile<CTAS>(a, w, BN_OUT, lane);
+      const Tile t = next;
+      next.rows = 0;
+      if (w + wstep < a.work) next = find_tile<CTAS>(a, w + wstep, BN_OUT, lane);
       if (t.rows == 0) continue;
       const int k0 = (int)((int64_t)a.kt * t.split / a.splits), k1 = (int)((int64_t)a.kt * (t.split + 1) / a.splits);
       const int rows = min(32, t.rows - rank * GM - quad * 32);     // of this warp; may be <= 0
@@ -545,15 +563,14 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS, FP8), 1) gemm_kernel(c
         if constexpr (MODE == GATED_GRAD) {
           uint32_t dh[16];
           load_chunk(dh, a.dh_vec, a.dh, a.n, row0, rows, out_col(c), a.n, stg + 2048, lane);
-          if (a.dh_vec) fetch_dh(c + 1 < NCH / 2 ? w : w + wstep, c + 1 < NCH / 2 ? c + 1 : 0);
+          if (a.dh_vec) fetch_dh(c + 1 < NCH / 2 ? t : next, c + 1 < NCH / 2 ? c + 1 : 0);
           auto grads = [&](auto type) {
             with_activation(a.act, [&](auto k) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) {
                 float lo, hi;
                 unpack16<decltype(type)::value>(dh[i], lo, hi);
-                gate_grads<decltype(k)::value>(lo, g[2 * i], u[2 * i]);
-                gate_grads<decltype(k)::value>(hi, g[2 * i + 1], u[2 * i + 1]);
+                gate_grads2<decltype(k)::value>(lo, hi, g[2 * i], g[2 * i + 1], u[2 * i], u[2 * i + 1]);
               }
             });
           };
@@ -569,7 +586,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS, FP8), 1) gemm_kernel(c
         }
         with_activation(a.act, [&](auto k) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) g[i] = activate<decltype(k)::value>(g[i]) * u[i];
+          for (int i = 0; i < 32; i += 2) gate2<decltype(k)::value>(g[i], g[i + 1], u[i], u[i + 1]);
         });
         if (!FP8 || !a.q) store_chunk(g, a.out_type, a.out_vec, a.out[0], a.ld_out, row0, rows, out_col(c), a.n, stg, lane);
       };
@@ -870,7 +887,7 @@ static Shape shape_of(const GemmCall &c) {
   const bool two = paired(c);
   const int64_t per = (c.k + ke - 1) / ke, wide = two ? 2 * c.n : c.n;
   const double size = c.fp8 ? 1.0 : 2.0, pairs = c.dual == DUAL_NONE ? 1.0 : 2.0;
-  const double bytes = (((c.dual == DUAL_CONCAT || (c.dual == DUAL_BATCH && c.m != c.n) ? 2.0 : 1.0) * c.m * c.k + pairs * c.types * c.n * c.k) * size);
+  const double bytes = ((two ? 1.0 : pairs) * c.m * c.k + pairs * c.types * c.n * c.k) * size;
   Shape best{};
   double best_us = 1e30;
   for (int bn = 256; bn >= 64; bn /= 2) {
@@ -953,6 +970,7 @@ int gemm(const GemmCall &c, const char *what, cudaStream_t stream) {
   const int64_t work = s.tiles_m * s.tiles_n * s.batch * s.splits;
   GPHL_REQUIRE(work + 65536 < INT32_MAX, "%s: too many tiles", what);
   a.m = c.m, a.n = c.n, a.tiles_m = (uint32_t)s.tiles_m, a.tiles_n = (uint32_t)s.tiles_n, a.work = (uint32_t)work;
+  a.by_plane.set(a.tiles_m * a.tiles_n), a.by_band.set(RASTER * a.tiles_n), a.by_last.set(a.tiles_m % RASTER ? a.tiles_m % RASTER : RASTER);
   a.batch = s.batch, a.splits = s.splits, a.kt = s.kt, a.kt_first = c.dual == DUAL_CONCAT ? s.kt / 2 : s.kt;
   a.a_mn = c.a_mn, a.b_mn = c.b_mn, a.types = (int32_t)c.types, a.ptr = c.ptr;
   a.idesc = (1u << 4) | ((uint32_t)(s.bn >> 3) << 17) | ((uint32_t)(GM * s.ctas >> 4) << 24);

@@ -101,6 +101,34 @@ template <int ACT> __device__ __forceinline__ void gate_grads(float dh, float &g
   }
   g = dh * u * d, u = dh * h;
 }
+// Two neighbouring elements at once: h = act(g) u, and the pair dg, du into g, u.  silu in packed arithmetic (one instruction for both
+// elements but for exponential and reciprocal).
+__device__ __forceinline__ uint64_t both(float v) { return pack2(v, v); }
+__device__ __forceinline__ uint64_t sigmoid2(uint64_t g) {
+  float a, b;
+  unpack2(fmul2(g, both(-LOG2E)), a, b);
+  unpack2(fadd2(pack2(exp2_fast(a), exp2_fast(b)), both(1.f)), a, b);
+  return pack2(rcp_fast(a), rcp_fast(b));
+}
+template <int ACT> __device__ __forceinline__ void gate2(float &g0, float &g1, float u0, float u1) {
+  if constexpr (ACT == ACT_SILU) {
+    const uint64_t g = pack2(g0, g1);
+    unpack2(fmul2(fmul2(g, sigmoid2(g)), pack2(u0, u1)), g0, g1);
+  } else {
+    g0 = activate<ACT>(g0) * u0, g1 = activate<ACT>(g1) * u1;
+  }
+}
+template <int ACT> __device__ __forceinline__ void gate_grads2(float dh0, float dh1, float &g0, float &g1, float &u0, float &u1) {
+  if constexpr (ACT == ACT_SILU) {
+    const uint64_t dh = pack2(dh0, dh1), g = pack2(g0, g1), s = sigmoid2(g), h = fmul2(g, s);
+    const uint64_t d = ffma2(h, fsub2(both(1.f), s), s);
+    unpack2(fmul2(fmul2(dh, pack2(u0, u1)), d), g0, g1);
+    unpack2(fmul2(dh, h), u0, u1);
+  } else {
+    gate_grads<ACT>(dh0, g0, u0);
+    gate_grads<ACT>(dh1, g1, u1);
+  }
+}
 // Calls f with the activation as a constant: the choice is made once for many elements (a branch an element, unrolled, also overran the
 // instruction cache: 300,000 x 256 -> 1024 in 1.11 ms).
 template <typename F> __device__ __forceinline__ void with_activation(int act, F f) {
