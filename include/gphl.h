@@ -293,6 +293,8 @@ int gphl_debug_reset_wait_timeouts(void); /* sets the counter back to 0 (synchro
 
 /* ---- dense operators of a transformer block on node rows --------------------------------------
  *
+ * Sums are fp32 (unlike the reductions above), in an order that depends on the sizes alone: results repeat bit for bit.
+ *
  * 8-bit rows ("codes"): e4m3 values with one fp32 scale per row and block of 128 columns, scale (row, b) at
  * scales[row * scale_row_stride + b * scale_block_stride]; code rows start on 16-byte boundaries.  The quantisers write
  * powers of two (the smallest 2^e >= 2^-126 with the block's largest finite magnitude <= 448 * 2^e), code rows padded with zeros to
