@@ -592,6 +592,8 @@ def _op(name: str):
         if not hasattr(torch.ops.my_ops, name):
             if not TORCH_OPS_LIB.exists():
                 raise GphlError(f"{TORCH_OPS_LIB} is missing: run `python -m graphiler_b200.build` (there is no fallback path)")
+            if hasattr(torch.ops.my_ops, "SpMMSrc"):      # a second registration of the same names would end the process
+                raise GphlError(f"the libgraphiler.so that is loaded has no {name}: install the present build in its place")
             torch.ops.load_library(str(TORCH_OPS_LIB))
         fn = _OPS[name] = getattr(torch.ops.my_ops, name).default
     return fn

@@ -880,6 +880,9 @@ struct Shape {
 // tiles, which read A more often), at least the time of the operands' bytes at the rate that tiles of that width were seen to stream them, and
 // for parts their join (3, and the parts' fp32 sums written and read at 5 TB/s).  In e4m3: 2048 x 11264 -> 4096 takes 112 with k whole, 141 in
 // 2 parts; 1 x 4096 -> 8192 18.7 in 2 parts, 14.0 in 4; 1 x 16384 -> 16384 73 with 128 columns a tile, 59 with 256 and 2 parts.
+// The tensor core truncates when it adds to an fp32 accumulator: over k values of one sign a sum loses 5.4e-9 k of itself (65,536: 3.5e-4,
+// 524,288: 3.0e-3), so in 16 bits no part is longer than CHAIN (1.8e-4, below half a step of the results); the join adds with rounding.
+constexpr int64_t CHAIN = 32768;
 static bool paired(const GemmCall &c) { return c.dual == DUAL_GATED || c.dual == DUAL_GATED_GRAD; }
 static Shape shape_of(const GemmCall &c) {
   const int ke = c.fp8 ? 128 : 64;
@@ -907,7 +910,8 @@ static Shape shape_of(const GemmCall &c) {
       const int64_t items = s.tiles_m * s.tiles_n * s.batch;
       const double rate = bn == 256 ? 5.2e6 : bn == 128 ? 4.0e6 : 3.2e6;      // bytes a microsecond
       const double step = bn == 256 ? (ctas == 1 ? 0.50 : c.fp8 ? 0.48 : 0.40) : bn == 128 ? 0.32 : 0.24;
-      for (int p = 1; p == 1 || (p <= 64 && p * 4 <= s.kt && items < 2 * units); ++p) {
+      const int least = c.fp8 ? 1 : (int)std::min<int64_t>(256, (s.kt * (int64_t)ke + CHAIN - 1) / CHAIN);
+      for (int p = least; p == least || (p <= 64 && p * 4 <= s.kt && items < 2 * units); ++p) {
         const double waves = (double)((items * p + units - 1) / units);
         double us = std::max(waves * ((double)s.kt / p * step + 1.5), bytes / rate);
         if (p > 1) us += 3.0 + (double)p * s.batch * c.m * wide * 8.0 / 5e6;

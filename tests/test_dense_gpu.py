@@ -292,6 +292,17 @@ def test_gated_fp8(m, k, f, act, dtype):
     assert ((got.scales.double() >= lo) & (got.scales.double() <= hi)).all()
 
 
+def test_long_sums_of_one_sign():
+    """131,072 positive terms: no chain of tensor-core additions (16 terms each) is longer than 2048, each loses at most 2^-23 of the sum."""
+    m, k = 2432, 131072
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w = (torch.rand(*s, generator=g, device="cuda").bfloat16() for s in ((m, k), (k, m)))
+    _, got, _ = capi().gated_linear(x, w, w, "relu", return_projections=True)
+    rows = torch.arange(0, m, 97, device="cuda")
+    want = sum(x[rows, a:a + 16384].double() @ w[a:a + 16384].double() for a in range(0, k, 16384))
+    assert float(((got[rows, :m].double() - want) / want).abs().max()) <= 2048 * 2.0 ** -23 + ref.FP32
+
+
 # ---- autograd -------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("shape", [(5, 64), (2, 3, 40), (257,)])
