@@ -131,8 +131,8 @@ struct NormGradArgs {
 // Rows are dealt to warps (or, for wpr > 1, to blocks) in turn; a lane keeps its columns, so dw gathers in its registers over all the
 // rows it meets and leaves once.  The next row's r and dy are on their way while a row is finished, and a lane holds 8 values of each, so
 // that 32 warps fit an SM.
-template <typename T, typename R>
-__global__ void __launch_bounds__(1024) rms_norm_grad_kernel(const NormGradArgs a) {
+template <typename T, typename R, int THREADS>
+__global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const NormGradArgs a) {
   constexpr int E = R::E, NV = 8 / E, RPW = 32 / R::LPR;
   __shared__ float s_part[32];
   extern __shared__ float s_dw[];                    // wpr == 1: n sums per row slot of the block
@@ -364,7 +364,8 @@ static GradShape grad_shape(int64_t m, int n, int e, int lpr, int sms) {
   }
   g.wpr = wpr, g.warps = wpr > 1 ? wpr : 8;
   const int slots = g.warps / g.wpr * (32 / lpr);
-  g.grid = (int)std::min<int64_t>((m + slots - 1) / slots, (int64_t)sms * (32 / g.warps));
+  // as many blocks as are resident (32 warps an SM, 16 with the wider registers of fp32 rows and single columns): the partial rows of dw stay few
+  g.grid = (int)std::min<int64_t>((m + slots - 1) / slots, (int64_t)sms * ((e == 4 && g.warps <= 16 ? 16 : 32) / g.warps));
   g.smem = g.wpr == 1 ? (size_t)slots * n * sizeof(float) : 0;
   return g;
 }
@@ -372,7 +373,10 @@ template <typename T, typename R> static void grad_launch(NormGradArgs a, int sm
   g = grad_shape(a.m, a.n, R::E, R::LPR, sms);
   a.wpr = g.wpr;
   if (g.wpr > 0) {
-    rms_norm_grad_kernel<T, R><<<g.grid, g.warps * 32, g.smem, s>>>(a);
+    // 64 registers a thread are enough for 16-bit rows; fp32 rows and single columns spill with them and get up to 128 (and fewer warps) while
+    // blocks are small enough
+    if (R::E == 4 && g.warps <= 16) rms_norm_grad_kernel<T, R, 512><<<g.grid, g.warps * 32, g.smem, s>>>(a);
+    else rms_norm_grad_kernel<T, R, 1024><<<g.grid, g.warps * 32, g.smem, s>>>(a);
   } else if constexpr (R::LPR == 32) {
     a.wpr = 16;
     rms_norm_grad_wide_kernel<T, R><<<(unsigned)a.m, 512, 0, s>>>(a);

@@ -911,7 +911,7 @@ static Shape shape_of(const GemmCall &c) {
       const double rate = bn == 256 ? 5.2e6 : bn == 128 ? 4.0e6 : 3.2e6;      // bytes a microsecond
       const double step = bn == 256 ? (ctas == 1 ? 0.50 : c.fp8 ? 0.48 : 0.40) : bn == 128 ? 0.32 : 0.24;
       const int least = c.fp8 ? 1 : (int)std::min<int64_t>(256, (s.kt * (int64_t)ke + CHAIN - 1) / CHAIN);
-      for (int p = least; p == least || (p <= 64 && p * 4 <= s.kt && items < 2 * units); ++p) {
+      for (int p = least; p == least || (p <= 64 && p * 4 <= s.kt && items < 2 * units && items * p <= 8 * units); ++p) {
         const double waves = (double)((items * p + units - 1) / units);
         double us = std::max(waves * ((double)s.kt / p * step + 1.5), bytes / rate);
         if (p > 1) us += 3.0 + (double)p * s.batch * c.m * wide * 8.0 / 5e6;
