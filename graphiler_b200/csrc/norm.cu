@@ -323,7 +323,7 @@ template <typename T, typename R, int NV, bool FP8> static void norm_launch(cons
   rms_norm_kernel<T, R, NV, FP8><<<(unsigned)((a.m + per_block - 1) / per_block), warps * 32, 0, s>>>(a);
 }
 template <typename T, typename R, bool FP8> static void norm_dispatch(NormArgs a, int sms, cudaStream_t s) {
-  constexpr int LOW = 8 / R::E, HIGH = 32 / R::E;    // steps a warp holds: 8 or 32 values a lane
+  constexpr int LOW = 8 / R::E, HIGH = 16 / R::E;    // steps a warp holds: 8 or 16 values a lane
   const int steps = (a.n + R::STEP - 1) / R::STEP;
   // Few warps a row leave most loads in flight per warp and need the fewest joins; when the rows would not fill the GPU with 8 warps an
   // SM that way, a row is spread over more warps instead.
