@@ -58,34 +58,42 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
   constexpr int KEEP = NV > 0 ? NV : 1;
   float v[KEEP][E];
   float ss = 0.f;
-  auto read = [&](int step, float (&t)[E]) {
-    R::load(x, step, lane, a.n, t);
+  // a step of r, from the inputs; stored where there is a residual
+  auto take = [&](typename R::Raw t, const typename R::Raw &u, int step, float (&f)[E]) {
+    R::widen(t, f);
     if (res) {
-      float u[E];
-      R::load(res, step, lane, a.n, u);
+      float g[E];
+      R::widen(u, g);
 #pragma unroll
-      for (int j = 0; j < E; ++j) t[j] = to_float(from_float<T>(t[j] + u[j]));
+      for (int j = 0; j < E; ++j) f[j] += g[j];
+      t = R::round(f);
+      R::widen(t, f);
+      if (r) R::store(r, step, lane, a.n, t);
     }
   };
   if constexpr (NV > 0) {
+    typename R::Raw xs[NV], rs[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int step = w0 + i * a.wpr;
-      if (step < steps) read(step, v[i]);
+      if (step < steps) {
+        xs[i] = R::raw(x, step, lane, a.n);
+        if (res) rs[i] = R::raw(res, step, lane, a.n);
+      }
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int step = w0 + i * a.wpr;
       if (step < steps) {
-        if (r) R::store(r, step, lane, a.n, v[i]);
+        take(xs[i], rs[i], step, v[i]);
 #pragma unroll
         for (int j = 0; j < E; ++j) ss = fmaf(v[i][j], v[i][j], ss);
       }
     }
   } else {
     for (int step = w0; step < steps; step += a.wpr) {
-      read(step, v[0]);
-      if (r) R::store(r, step, lane, a.n, v[0]);
+      const typename R::Raw t = R::raw(x, step, lane, a.n);
+      take(t, res ? R::raw(res, step, lane, a.n) : t, step, v[0]);
       float part = 0.f;
 #pragma unroll
       for (int j = 0; j < E; ++j) part = fmaf(v[0][j], v[0][j], part);
@@ -97,8 +105,7 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
 
   auto write = [&](int step, const float (&t)[E]) {
     float w[E], y[E];
-    if (a.w_f32) R::load(static_cast<const float *>(a.w), step, lane, a.n, w);
-    else R::load(static_cast<const T *>(a.w), step, lane, a.n, w);
+    R::weight(a.w, a.w_f32, step, lane, a.n, w);
 #pragma unroll
     for (int j = 0; j < E; ++j) y[j] = t[j] * rstd * w[j];
     if constexpr (FP8) store_codes<R>(y, a.q + row * a.n_pad, a.scales + row, a.scale_stride, step, lane, a.n, a.n_pad, live);
@@ -112,8 +119,8 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
     }
   } else {
     for (int step = w0; step < steps; step += a.wpr) {
-      if (r) R::load(r, step, lane, a.n, v[0]);      // this thread's own stores
-      else read(step, v[0]);
+      const typename R::Raw t = R::raw(r ? r : x, step, lane, a.n);      // r: this thread's own stores
+      R::widen(t, v[0]);
       write(step, v[0]);
     }
   }
@@ -179,8 +186,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_grad_kernel(const NormGradAr
         float w[E], part = 0.f;
         R::widen(r[i], xh[i]);
         R::widen(dy[i], g[i]);
-        if (a.w_f32) R::load(static_cast<const float *>(a.w), step, lane, a.n, w);
-        else R::load(static_cast<const T *>(a.w), step, lane, a.n, w);
+        R::weight(a.w, a.w_f32, step, lane, a.n, w);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
           xh[i][j] *= scale;
@@ -248,10 +254,9 @@ __global__ void __launch_bounds__(512) rms_norm_grad_wide_kernel(const NormGradA
   const float rstd = __ldg(a.rstd + row);
   float xh[E], g[E], w[E];
   auto read = [&](int step) {
-    R::load(r, step, lane, a.n, xh);
-    R::load(dy, step, lane, a.n, g);
-    if (a.w_f32) R::load(static_cast<const float *>(a.w), step, lane, a.n, w);
-    else R::load(static_cast<const T *>(a.w), step, lane, a.n, w);
+    R::widen(R::raw(r, step, lane, a.n), xh);
+    R::widen(R::raw(dy, step, lane, a.n), g);
+    R::weight(a.w, a.w_f32, step, lane, a.n, w);
 #pragma unroll
     for (int j = 0; j < E; ++j) xh[j] *= rstd, g[j] *= w[j];
   };
@@ -267,7 +272,7 @@ __global__ void __launch_bounds__(512) rms_norm_grad_wide_kernel(const NormGradA
   for (int step = warp; step < steps; step += a.wpr) {
     read(step);
     float o[E];
-    if (dr) R::load(dr, step, lane, a.n, o);
+    if (dr) R::widen(R::raw(dr, step, lane, a.n), o);
 #pragma unroll
     for (int j = 0; j < E; ++j) {
       const float t = rstd * fmaf(-xh[j], mean, g[j]);
@@ -325,9 +330,10 @@ template <typename T, typename R, int NV, bool FP8> static void norm_launch(cons
 template <typename T, typename R, bool FP8> static void norm_dispatch(NormArgs a, int sms, cudaStream_t s) {
   constexpr int LOW = 8 / R::E, HIGH = 16 / R::E;    // steps a warp holds: 8 or 16 values a lane
   const int steps = (a.n + R::STEP - 1) / R::STEP;
-  // Few warps a row leave most loads in flight per warp and need the fewest joins; when the rows would not fill the GPU with 8 warps an
-  // SM that way, a row is spread over more warps instead.
-  int wpr = pow2_at_least((steps + HIGH - 1) / HIGH);
+  // Few warps a row leave most loads in flight per warp and need the fewest joins (16 values a lane: 100,000 x 1024 in bf16 128 us, 8 values
+  // 149); when the rows would not fill the GPU with 8 warps an SM that way, and for single columns (10007 x 1001 fp32: 29 against 31 us), a
+  // row is spread over more warps instead.
+  int wpr = pow2_at_least(R::SINGLE ? (steps + LOW - 1) / LOW : (steps + HIGH - 1) / HIGH);
   if (a.m * wpr < 8 * sms) wpr = pow2_at_least((steps + LOW - 1) / LOW);
   a.wpr = std::min(wpr, 16);
   const int warps = a.wpr == 1 ? 4 : a.wpr;

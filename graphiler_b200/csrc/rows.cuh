@@ -55,57 +55,66 @@ template <typename T, bool SC, int LPR_ = 32> struct Row {
       for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(x.w[j]);
     } else {
 #pragma unroll
+      for (int j = 0; j < 4; ++j) widen2(x.w[j], v[2 * j], v[2 * j + 1]);
+    }
+  }
+  // Two 16-bit values of a word, and back (one instruction for the pair).
+  __device__ static __forceinline__ void widen2(uint32_t w, float &lo, float &hi) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+      lo = f.x, hi = f.y;
+    }
+  }
+  // Rounded to T as stored (single columns: the rounded values, widened).
+  __device__ static __forceinline__ Raw round(const float (&v)[E]) {
+    Raw x;
+    if constexpr (E == 4) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x.w[j] = __float_as_uint(to_float(from_float<T>(v[j])));
+    } else {
+#pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          v[2 * j] = __uint_as_float(x.w[j] << 16), v[2 * j + 1] = __uint_as_float(x.w[j] & 0xffff0000u);
+          const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          x.w[j] = *reinterpret_cast<const uint32_t *>(&h);
         } else {
-          const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&x.w[j]));
-          v[2 * j] = f.x, v[2 * j + 1] = f.y;
+          const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+          x.w[j] = *reinterpret_cast<const uint32_t *>(&h);
         }
       }
     }
+    return x;
   }
-  // U: the stored type, T or float (a weight kept in 32 bits beside 16-bit rows)
-  template <typename U> __device__ static __forceinline__ void load(const U *__restrict__ row, int step, int lane, int n, float (&v)[E]) {
+  __device__ static __forceinline__ void store(T *__restrict__ row, int step, int lane, int n, const Raw &x) {
     if constexpr (SC) {
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const int c = col(step, lane, j);
-        v[j] = c < n ? to_float(row[c]) : 0.f;
+        if (c < n) row[c] = from_float<T>(__uint_as_float(x.w[j]));      // rounded already
       }
     } else {
-      constexpr int PER = 16 / (int)sizeof(U);        // values of one 16-byte load
       const int c = col(step, lane, 0);
-      if (c < n) {
-#pragma unroll
-        for (int q = 0; q < E / PER; ++q) {
-          const uint4 raw = *reinterpret_cast<const uint4 *>(row + c + q * PER);
-          const U *p = reinterpret_cast<const U *>(&raw);
-#pragma unroll
-          for (int j = 0; j < PER; ++j) v[q * PER + j] = to_float(p[j]);
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < E; ++j) v[j] = 0.f;
-      }
+      if (c < n) *reinterpret_cast<uint4 *>(row + c) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
     }
   }
-  __device__ static __forceinline__ void store(T *__restrict__ row, int step, int lane, int n, const float (&v)[E]) {
-    if constexpr (SC) {
+  __device__ static __forceinline__ void store(T *__restrict__ row, int step, int lane, int n, const float (&v)[E]) { store(row, step, lane, n, round(v)); }
+  // A weight row kept as T or, `f32`, in 32 bits.
+  __device__ static __forceinline__ void weight(const void *w, bool f32, int step, int lane, int n, float (&v)[E]) {
+    if (!f32) {
+      widen(raw(static_cast<const T *>(w), step, lane, n), v);
+    } else if constexpr (E == 4) {                     // single columns, or T is float
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
+      for (int j = 0; j < 4; ++j) {
         const int c = col(step, lane, j);
-        if (c < n) row[c] = from_float<T>(v[j]);
+        v[j] = c < n ? static_cast<const float *>(w)[c] : 0.f;
       }
     } else {
       const int c = col(step, lane, 0);
-      if (c < n) {
-        uint4 raw;
-        T *p = reinterpret_cast<T *>(&raw);
-#pragma unroll
-        for (int j = 0; j < E; ++j) p[j] = from_float<T>(v[j]);
-        *reinterpret_cast<uint4 *>(row + c) = raw;
-      }
+      const float *p = static_cast<const float *>(w) + c;
+      const float4 a = c < n ? *reinterpret_cast<const float4 *>(p) : make_float4(0, 0, 0, 0), b = c < n ? *reinterpret_cast<const float4 *>(p + 4) : a;
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
     }
   }
 };
