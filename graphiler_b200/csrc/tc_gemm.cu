@@ -398,6 +398,7 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS, FP8), 1) gemm_kernel(c
   constexpr int KE = FP8 ? 128 : 64;                     // k of a step
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t s_full[MAX_STAGES], s_empty[MAX_STAGES], s_acc_full[2], s_acc_empty[2], s_pair[4], s_drain;
+  __shared__ int8_t s_exp[2][FP8 ? EPI_WARPS : 1][32];   // codes: the exponent of a row's scale as each warp sees it, in -126 .. 120
   __shared__ uint32_t s_tmem;
   __shared__ int s_failed;
 
@@ -683,17 +684,17 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS, FP8), 1) gemm_kernel(c
             for (int c = 0; c < NCH / 2; ++c)
 #pragma unroll
               for (int i = 0; i < 32; ++i) big = fmaxf(big, out_col(c) + i < a.n ? finite_abs(g[c][i]) : 0.f);
-            // (two slots in turn: a slot is written again only after the others' next arrivals, which follow their reads)
-            const uint32_t slot = 2048 + (tiles & 1) * 128;
-            reinterpret_cast<float *>(stg + slot)[lane] = big;
+            // Joined as exponents, in memory of their own (the staging buffer's row scales of the next tile may be on their way before the other warp
+            // has read).  Two slots in turn: one is written again only after the others' next arrivals, which follow their reads.
+            int e = fp8_exponent(big);
+            s_exp[tiles & 1][warp][lane] = (int8_t)e;
             __syncwarp();
             if (lane == 0) tc::arrive<1>(pair + 8 * quad);
             ok = __all_sync(FULL, tc::mbar_wait(pair + 8 * quad, tiles & 1, failed));
             if (!ok) break;
-            ++tiles;
 #pragma unroll
-            for (int i = 0; i < PARTS; ++i) big = fmaxf(big, reinterpret_cast<const float *>(ring + RING_BYTES + (quad + 4 * i) * STAGING + slot)[lane]);
-            const int e = fp8_exponent(big);
+            for (int i = 0; i < PARTS; ++i) e = max(e, (int)s_exp[tiles & 1][quad + 4 * i][lane]);
+            ++tiles;
             if (cpart == 0 && lane < rows) a.q_scale[(int64_t)(t.n0 / 128) * a.q_scale_stride + row0 + lane] = pow2f(e);
 #pragma unroll
             for (int c = 0; c < NCH / 2; ++c) store_code_chunk(g[c], pow2f(-e), a.q, a.ld_out, row0, rows, out_col(c), a.n, stg, lane);

@@ -509,6 +509,19 @@ def test_results_repeat_bit_for_bit():
     assert all(torch.equal(a, b) for a, b in zip(first, c.rms_norm_grad(r, w, rstd, x)))
 
 
+def test_codes_repeat_over_many_tiles():
+    """Long k and more tiles than blocks: the warps that share a row's scale run ahead of one another into the next tile."""
+    c = capi()
+    x, wg, wu = codes(1000, 2600, 1), weights(1, 2600, 6000, 2), weights(1, 2600, 6000, 3)
+    first = c.gated_linear_fp8(x, wg, wu)
+    h = c.gated_linear_fp8(x, wg, wu, out_dtype=F32)
+    want = c.quantize_fp8(h)                       # the same fp32 values, quantised by themselves
+    for _ in range(20):
+        got = c.gated_linear_fp8(x, wg, wu)
+        assert torch.equal(got.values.view(torch.uint8), first.values.view(torch.uint8)) and torch.equal(got.scales, first.scales)
+    assert torch.equal(first.scales, want.scales) and torch.equal(first.values.view(torch.uint8), want.values.view(torch.uint8))
+
+
 def test_no_wait_ran_out():
     assert capi().tc_wait_timeouts() == 0
 
