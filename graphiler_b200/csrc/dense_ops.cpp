@@ -143,13 +143,29 @@ bool wants_grad(std::initializer_list<const Tensor *> ts) {
   return false;
 }
 
+// A captured backward pass must not reach gradients that belong to another stream: the engine would make that stream wait for the capture,
+// which ends the process.  An input's gradient belongs to the stream of the graph that it is part of: for a leaf, of any living graph.
+void capturable(std::initializer_list<const Tensor *> ts, const char *what) {
+  if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
+  for (const Tensor *t : ts) {
+    if (!t->defined() || !t->requires_grad()) continue;
+    const auto node = t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn();
+    const auto stream = node ? node->stream() : std::nullopt;
+    TORCH_CHECK(!stream || *stream == at::cuda::getCurrentCUDAStream(t->get_device()).unwrap(), what,
+                ": an input's gradients belong to a graph that was recorded on another stream than the one that is captured (drop that graph's outputs first)");
+  }
+}
+
 std::vector<Tensor> rms_norm(const Tensor &x, const Tensor &w, double eps, const OptTensor &res_) {
   const Tensor res = res_.value_or(Tensor());
   TORCH_CHECK(x.dim() >= 1 && w.dim() == 1 && x.size(-1) == w.size(0), "rms_norm needs rows (..., n) and a weight of n values");
   TORCH_CHECK(!res.defined() || res.sizes() == x.sizes(), "rms_norm: the residual must have the rows' shape and type");
   on_device({&x, &w, &res});
   const Tensor wc = w.contiguous();
-  if (wants_grad({&x, &w, &res})) return RmsNorm::apply(x, wc, eps, res_);
+  if (wants_grad({&x, &w, &res})) {
+    capturable({&x, &w, &res}, "rms_norm");
+    return RmsNorm::apply(x, wc, eps, res_);
+  }
   auto [y, r, rstd] = norm_run(rows_of(x), wc, eps, res.defined() ? rows_of(res) : res, false);
   std::vector<Tensor> out{y.view(x.sizes())};
   if (r.defined()) out.push_back(r.view(x.sizes()));
@@ -387,7 +403,10 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
 Tensor gated_linear(const Tensor &x, const Tensor &wg, const Tensor &wu, c10::string_view act) {
   TORCH_CHECK(x.dim() >= 1 && wg.dim() == 2 && x.size(-1) == wg.size(0), "gated_linear needs rows (..., k) and two weights (k, f)");
   on_device({&x, &wg, &wu});
-  if (wants_grad({&x, &wg, &wu})) return GatedLinear::apply(x, wg, wu, std::string(act));
+  if (wants_grad({&x, &wg, &wu})) {
+    capturable({&x, &wg, &wu}, "gated_linear");
+    return GatedLinear::apply(x, wg, wu, std::string(act));
+  }
   auto shape = x.sizes().vec();
   shape.back() = wg.size(1);
   return std::get<0>(gated_run(rows_of(x), wg, wu, act, false)).view(shape);

@@ -498,6 +498,36 @@ def test_captured_training_step():
     del g
 
 
+def test_capture_beside_a_living_graph_is_refused():
+    """An eager graph of the same leaves lives: a captured backward pass would reach its stream."""
+    from graphiler_b200 import capi as c, dense
+    x, wg, wu, dh = gated_inputs(40, 96, 128, BF16, False)
+    nw = torch.ones(96, device="cuda", dtype=BF16).requires_grad_(True)
+    wg.requires_grad_(True)
+    kept = dense.gated_linear(dense.rms_norm(x, nw), wg, wu)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = x + 1
+        with pytest.raises(c.GphlError, match="another stream"):
+            dense.rms_norm(x, nw)
+        with pytest.raises(c.GphlError, match="another stream"):
+            dense.gated_linear(x, wg, wu)
+        with torch.no_grad():
+            h = dense.gated_linear(x, wg, wu)
+    g.replay()
+    torch.cuda.synchronize()
+    with torch.no_grad():
+        assert torch.equal(h, dense.gated_linear(x, wg, wu)) and torch.equal(y, x + 1)
+    del kept, g
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dw, dn = torch.autograd.grad(dense.gated_linear(dense.rms_norm(x, nw), wg, wu), (wg, nw), dh)
+    g.replay()
+    want = torch.autograd.grad(dense.gated_linear(dense.rms_norm(x, nw), wg, wu), (wg, nw), dh)
+    assert torch.equal(dw, want[0]) and torch.equal(dn, want[1])
+    del g
+
+
 def test_results_repeat_bit_for_bit():
     c = capi()
     x, wg, wu, dh = gated_inputs(1500, 96, 264, BF16, False)
