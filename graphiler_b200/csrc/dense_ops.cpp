@@ -3,6 +3,7 @@
 // caching allocator (a captured call's scratch is private to its graph), launch on the current stream.  `rms_norm` and
 // `gated_linear` are differentiable; the others record no gradients.  No counterpart in the reference's registry.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
@@ -47,10 +48,16 @@ void on_device(std::initializer_list<const Tensor *> ts) {
 void contiguous(std::initializer_list<const Tensor *> ts) {
   for (const Tensor *t : ts) TORCH_CHECK(!t || !t->defined() || t->is_contiguous(), "operators need contiguous tensors");
 }
-Tensor scratch(int64_t bytes, const Tensor &like) {
-  return bytes > 0 ? torch::empty({bytes}, like.options().dtype(torch::kUInt8).requires_grad(false)) : Tensor();
+// New memory beside `t`, straight from the caching allocator: through the dispatcher each tensor and each view of it costs the host a microsecond.
+Tensor plain(const Tensor &t, torch::ScalarType s, at::IntArrayRef shape) { return Tensor(at::detail::empty_cuda(shape, s, t.device(), c10::nullopt)); }
+// A tensor made here and not yet handed out, seen with other sizes and strides.
+Tensor as(Tensor t, at::IntArrayRef sizes, at::IntArrayRef strides) {
+  t.unsafeGetTensorImpl()->set_sizes_and_strides(sizes, strides);
+  return t;
 }
-Tensor plain(const Tensor &t, torch::ScalarType s, at::IntArrayRef shape) { return torch::empty(shape, t.options().dtype(s).requires_grad(false)); }
+Tensor scratch(int64_t bytes, const Tensor &like) {
+  return bytes > 0 ? plain(like, torch::kUInt8, {bytes}) : Tensor();
+}
 
 // ---- norm -------------------------------------------------------------------------------------------------------
 
@@ -179,7 +186,8 @@ struct Codes {
 };
 // Empty codes as the quantisers lay them out: rows padded to 16 bytes, a block's scales of consecutive rows together.
 Codes new_rows(int64_t m, int64_t n, const Tensor &like) {
-  return {plain(like, torch::kFloat8_e4m3fn, {m, up(n, 16)}).slice(1, 0, n), plain(like, torch::kFloat32, {up(n, BLOCK) / BLOCK, m}).t()};
+  const int64_t row = up(n, 16), blocks = up(n, BLOCK) / BLOCK;
+  return {as(plain(like, torch::kFloat8_e4m3fn, {m, row}), {m, n}, {row, 1}), as(plain(like, torch::kFloat32, {blocks, m}), {m, blocks}, {1, m})};
 }
 
 std::vector<Tensor> rms_norm_fp8(const Tensor &x, const Tensor &w, double eps, const OptTensor &res_) {
