@@ -22,7 +22,7 @@ CSRC = PKG / "csrc"
 LIB = PKG / "lib"
 
 KERNEL_SOURCES = ["plan.cu", "spmm.cu", "softmax.cu", "sddmm.cu", "gather.cu", "segment_mm.cu", "segment_mm_tc.cu", "gspmm.cu",
-                  "norm.cu", "fp8.cu", "tc_gemm.cu", "gated.cu"]
+                  "norm.cu", "fp8.cu", "tc_gemm.cu", "few_rows.cu", "gated.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 

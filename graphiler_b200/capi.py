@@ -569,7 +569,7 @@ def linear_fanout(x, w, fan: FanOut, row_scale=None, relu: bool = False, out=Non
 # These go through the TorchScript registrations (csrc/dense_ops.cpp) instead of ctypes: a call of few rows is bound by the host.
 
 class Fp8Rows(NamedTuple):
-    """Rows in 8 bits: e4m3 ``values`` (m, k), rows starting on 16-byte boundaries, and float32 ``scales`` (m, ceil(k / 128)) of any
+    """Rows in 8 bits: e4m3 ``values`` (m, k), rows starting on 16-byte boundaries (padded to them, the last one too), and float32 ``scales`` (m, ceil(k / 128)) of any
     strides, one per row and block of 128 columns; a value stands for ``values * scale``."""
     values: torch.Tensor
     scales: torch.Tensor

@@ -245,6 +245,8 @@ int64_t code_rows(const Tensor &q, const Tensor &s, int64_t dim, const char *wha
   const int64_t row = n > 1 ? q.stride(-2) : several ? q.stride(0) : up(k, 16);
   TORCH_CHECK((k == 1 || q.stride(-1) == 1) && row % 16 == 0 && row >= k && (!several || q.stride(0) == n * row) && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
               what, ": rows of codes must be contiguous and start on 16-byte boundaries, equally far apart (as the quantisers lay them out)");
+  // the last row's padding is read too (and counts for nothing)
+  TORCH_CHECK((q.storage_offset() + (q.numel() / k - 1) * row + up(k, 16)) <= (int64_t)q.storage().nbytes(), what, ": the last row of codes must be padded to 16 bytes like the others");
   return row;
 }
 

@@ -885,10 +885,13 @@ struct Shape {
 // 524,288: 3.0e-3), so in 16 bits no part is longer than CHAIN (1.8e-4, below half a step of the results); the join adds with rounding.
 constexpr int64_t CHAIN = 32768;
 static bool paired(const GemmCall &c) { return c.dual == DUAL_GATED || c.dual == DUAL_GATED_GRAD; }
-static Shape shape_of(const GemmCall &c) {
-  const int ke = c.fp8 ? 128 : 64;
+static int sm_count() {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+static Shape shape_of(const GemmCall &c, int sms) {
+  const int ke = c.fp8 ? 128 : 64;
   const bool two = paired(c);
   const int64_t per = (c.k + ke - 1) / ke, wide = two ? 2 * c.n : c.n;
   const double size = c.fp8 ? 1.0 : 2.0, pairs = c.dual == DUAL_NONE ? 1.0 : 2.0;
@@ -926,7 +929,9 @@ static int64_t part_ld(const GemmCall &c) { return (c.n + 3) / 4 * 4 * (paired(c
 
 int64_t gemm_workspace_bytes(const GemmCall &c) {
   if (c.m <= 0 || c.n <= 0 || c.k <= 0) return 0;
-  const Shape s = shape_of(c);
+  const int few = few_rows_parts(c);
+  if (few >= 0) return (int64_t)few * c.m * part_ld(c) * (int64_t)sizeof(float);
+  const Shape s = shape_of(c, sm_count());
   return s.splits > 1 ? (int64_t)s.splits * s.batch * c.m * part_ld(c) * (int64_t)sizeof(float) : 0;
 }
 
@@ -955,11 +960,40 @@ template <bool FP8, int MODE> static int run_shape(const Shape &s, const GemmArg
   return run<128, 1, 8, FP8, MODE>(a, sms, stream);
 }
 
-int gemm(const GemmCall &c, const char *what, cudaStream_t stream) {
-  if (!encode_fn()) return fail(GPHL_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", what);
-  const Shape s = shape_of(c);
-  const bool pairs_of_b = paired(c);
+// What finishes a tile, or joins parts.
+static GemmArgs finish_args(const GemmCall &c) {
   GemmArgs a{};
+  a.m = c.m, a.n = c.n, a.batch = c.dual == DUAL_BATCH ? 2 : 1, a.types = (int32_t)c.types, a.ptr = c.ptr;
+  a.out[0] = c.out[0], a.out[1] = c.out[1], a.ld_out = c.ld_out, a.out_type = c.out_type, a.act = c.act;
+  a.out_vec = aligned16(c.out[0]) && aligned16(c.out[1]) && (c.ld_out * (c.out_type == GPHL_F32 ? 4 : 2)) % 16 == 0;
+  a.dh = c.dh, a.dh_vec = aligned16(c.dh) && c.n % 8 == 0;
+  a.g = c.g, a.u = c.u, a.ld_gu = c.ld_gu, a.q = c.q, a.q_scale = c.q_scale, a.q_scale_stride = c.q_scale_stride;
+  a.part = static_cast<float *>(c.workspace), a.ld_part = part_ld(c), a.part_u = (c.n + 3) / 4 * 4;
+  return a;
+}
+static int join(const GemmCall &c, GemmArgs &a, int parts, cudaStream_t stream) {
+  a.splits = parts;
+  const unsigned blocks = (unsigned)((a.batch * c.m * ((c.n + 127) / 128) + 7) / 8);
+  if (c.dual == DUAL_GATED_GRAD) gemm_join_kernel<GATED_GRAD><<<blocks, 256, 0, stream>>>(a);
+  else if (c.dual == DUAL_GATED) gemm_join_kernel<GATED><<<blocks, 256, 0, stream>>>(a);
+  else gemm_join_kernel<LINEAR><<<blocks, 256, 0, stream>>>(a);
+  return launched("gemm_join_kernel");
+}
+
+int gemm(const GemmCall &c, const char *what, cudaStream_t stream) {
+  int dev = 0, sms = 0;
+  GPHL_CUDA(cudaGetDevice(&dev));
+  GPHL_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  GemmArgs a = finish_args(c);
+  const int few = few_rows_parts(c);
+  if (few >= 0) {
+    GPHL_REQUIRE(few == 0 || (a.part && aligned16(a.part)), "%s: the workspace is missing or not 16-byte aligned", what);
+    const int rc = few_rows(c, a.part, a.ld_part, a.part_u, what, stream);
+    return rc != GPHL_OK || few == 0 ? rc : join(c, a, few, stream);
+  }
+  if (!encode_fn()) return fail(GPHL_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", what);
+  const Shape s = shape_of(c, sms);
+  const bool pairs_of_b = paired(c);
   const int pairs = c.dual == DUAL_NONE ? 1 : 2;
   // With fewer rows than a tile, only they are brought: the tensor core multiplies whatever the stage's other rows hold into rows of the
   // accumulator that nobody reads.  (A box of 128 rows costs its time even where it is zeros: 5 x 4096 -> 11264 47 us.)
@@ -975,34 +1009,21 @@ int gemm(const GemmCall &c, const char *what, cudaStream_t stream) {
   }
   const int64_t work = s.tiles_m * s.tiles_n * s.batch * s.splits;
   GPHL_REQUIRE(work + 65536 < INT32_MAX, "%s: too many tiles", what);
-  a.m = c.m, a.n = c.n, a.tiles_m = (uint32_t)s.tiles_m, a.tiles_n = (uint32_t)s.tiles_n, a.work = (uint32_t)work;
+  a.tiles_m = (uint32_t)s.tiles_m, a.tiles_n = (uint32_t)s.tiles_n, a.work = (uint32_t)work;
   a.by_plane.set(a.tiles_m * a.tiles_n), a.by_band.set(RASTER * a.tiles_n), a.by_last.set(a.tiles_m % RASTER ? a.tiles_m % RASTER : RASTER);
-  a.batch = s.batch, a.splits = s.splits, a.kt = s.kt, a.kt_first = c.dual == DUAL_CONCAT ? s.kt / 2 : s.kt;
-  a.a_mn = c.a_mn, a.b_mn = c.b_mn, a.types = (int32_t)c.types, a.ptr = c.ptr;
+  a.splits = s.splits, a.kt = s.kt, a.kt_first = c.dual == DUAL_CONCAT ? s.kt / 2 : s.kt;
+  a.a_mn = c.a_mn, a.b_mn = c.b_mn;
   a.idesc = (1u << 4) | ((uint32_t)(s.bn >> 3) << 17) | ((uint32_t)(GM * s.ctas >> 4) << 24);
   if (!c.fp8) a.idesc |= (c.in_type == GPHL_BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)c.a_mn << 15) | ((uint32_t)c.b_mn << 16);
-  a.out[0] = c.out[0], a.out[1] = c.out[1], a.ld_out = c.ld_out, a.out_type = c.out_type, a.act = c.act;
-  a.out_vec = aligned16(c.out[0]) && aligned16(c.out[1]) && (c.ld_out * (c.out_type == GPHL_F32 ? 4 : 2)) % 16 == 0;
-  a.dh = c.dh, a.dh_vec = aligned16(c.dh) && c.n % 8 == 0;
-  a.g = c.g, a.u = c.u, a.ld_gu = c.ld_gu, a.q = c.q, a.q_scale = c.q_scale, a.q_scale_stride = c.q_scale_stride;
-  a.part = static_cast<float *>(c.workspace), a.ld_part = part_ld(c), a.part_u = (c.n + 3) / 4 * 4;
   a.a_scale = c.a_scale, a.b_scale[0] = c.b_scale[0], a.b_scale[1] = c.b_scale[1];
   a.a_scale_row = c.a_scale_row, a.a_scale_block = c.a_scale_block;
   a.scale_kb = (int32_t)((c.k + 127) / 128), a.scale_nb = (int32_t)((c.n + 127) / 128);
   GPHL_REQUIRE(s.splits == 1 || (a.part && aligned16(a.part)), "%s: the workspace is missing or not 16-byte aligned", what);
-  int dev = 0, sms = 0;
-  GPHL_CUDA(cudaGetDevice(&dev));
-  GPHL_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   int rc;
   if (c.dual == DUAL_GATED_GRAD) rc = run_shape<false, GATED_GRAD>(s, a, sms, stream);
   else if (c.dual == DUAL_GATED) rc = c.fp8 ? run_shape<true, GATED>(s, a, sms, stream) : run_shape<false, GATED>(s, a, sms, stream);
   else rc = c.fp8 ? run_shape<true, LINEAR>(s, a, sms, stream) : run_shape<false, LINEAR>(s, a, sms, stream);
-  if (rc != GPHL_OK || s.splits == 1) return rc;
-  const unsigned blocks = (unsigned)((s.batch * c.m * ((c.n + 127) / 128) + 7) / 8);
-  if (c.dual == DUAL_GATED_GRAD) gemm_join_kernel<GATED_GRAD><<<blocks, 256, 0, stream>>>(a);
-  else if (c.dual == DUAL_GATED) gemm_join_kernel<GATED><<<blocks, 256, 0, stream>>>(a);
-  else gemm_join_kernel<LINEAR><<<blocks, 256, 0, stream>>>(a);
-  return launched("gemm_join_kernel");
+  return rc != GPHL_OK || s.splits == 1 ? rc : join(c, a, s.splits, stream);
 }
 
 int gemm_wait_timeouts(int *count) {

@@ -51,6 +51,9 @@ struct GemmCall {
 
 int64_t gemm_workspace_bytes(const GemmCall &c);
 int gemm(const GemmCall &c, const char *what, cudaStream_t stream);
+// few_rows.cu: e4m3 products of few rows, without tiles.
+int few_rows_parts(const GemmCall &c);
+int few_rows(const GemmCall &c, float *part, int64_t ld_part, int64_t part_u, const char *what, cudaStream_t stream);
 int gemm_wait_timeouts(int *count);
 int gemm_reset_wait_timeouts();
 

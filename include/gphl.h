@@ -300,7 +300,8 @@ int gphl_debug_reset_wait_timeouts(void); /* sets the counter back to 0 (synchro
  * powers of two (the smallest 2^e >= 2^-126 with the block's largest finite magnitude <= 448 * 2^e), code rows padded with zeros to
  * q_stride = n rounded up to 16, and scale (row, b) at b * scale_stride + row; a non-finite value becomes the NaN code.  The product
  * takes any scales.  8-bit weights: w (n_types, n, k) codes, k contiguous and padded to a multiple of 16, with one scale per
- * 128 x 128 values, (n_types, ceil(n / 128), ceil(k / 128)) contiguous.
+ * 128 x 128 values, (n_types, ceil(n / 128), ceil(k / 128)) contiguous.  What the padding of code rows holds counts for nothing, but it
+ * must be there, behind the last row too.
  */
 
 /* r = round(x + residual) in the rows' type (r = x without a residual; then r may be NULL), y = r * rstd * w with
@@ -328,7 +329,7 @@ int gphl_quantize_fp8_weight(int32_t dtype, int64_t n_types, int64_t k, int64_t 
 int gphl_dequantize_fp8(int32_t dtype, int64_t m, int64_t n, const void *q, int64_t q_stride, const float *scales, int64_t scale_row_stride,
                         int64_t scale_block_stride, void *y, void *stream);
 
-/* Rows of 16-bit values (m, n), contiguous, copied to rows 16-byte aligned (n_pad = n rounded up to 8; the padding is not written):
+/* Rows of 16-bit values (m, n), contiguous, copied to rows 16-byte aligned (n_pad = n rounded up to 8; the padding is zeros):
  * the products below read their 16-bit operands in rows that start on 16-byte boundaries. */
 int gphl_pad_rows_16(int64_t m, int64_t n, const void *x, void *y, void *stream);
 

@@ -195,6 +195,42 @@ def test_mm_fp8_many_types():
     check_mm(codes(ptr[-1], 256, 10), weights(100, 256, 48, 20), ptr, F16)
 
 
+def nan_padding(c, q):
+    """The same codes in rows whose padding holds the NaN code."""
+    k = q.values.shape[-1]
+    wide = torch.full((*q.values.shape[:-1], (k + 15) // 16 * 16 + 16), 0x7f, dtype=torch.uint8, device="cuda")
+    wide[..., :k] = q.values.view(torch.uint8)
+    return type(q)(wide.view(torch.float8_e4m3fn)[..., :k], q.scales)
+
+
+@pytest.mark.parametrize("m", [1, 2, 7, 8, 9, 15, 16, 17])
+@pytest.mark.parametrize("k,n", [(1, 17), (15, 8), (130, 129), (1000, 300), (1024, 16), (3200, 1001)])
+def test_fp8_few_rows(m, k, n):
+    """Single tokens and small batches, whatever the rows' padding holds; the gated form too."""
+    c = capi()
+    x, w, wu = nan_padding(c, codes(m, k, 10)), nan_padding(c, weights(1, k, n, 20)), nan_padding(c, weights(1, k, n, 30))
+    y = check_mm(x, w, None, F16)
+    check_mm(x, w, None, F32)
+    assert torch.equal(y, c.segment_mm_fp8(c.Fp8Rows(x.values, x.scales.contiguous()), w, out_dtype=F16))
+    h = c.gated_linear_fp8(x, w, wu, "relu", out_dtype=F32)
+    xv, gv, uv = ref.rows_value(x), ref.weight_value(w)[0].t(), ref.weight_value(wu)[0].t()
+    g, u, loss = xv @ gv, xv @ uv, ref.sum_loss(k, fp8=True)
+    dg, du = loss * (xv.abs() @ gv.abs()), loss * (xv.abs() @ uv.abs())
+    ref.close(h, g.clamp(min=0) * u, dg * u.abs() + du * g.abs() + dg * du + 2.0 ** -22 * (g * u).abs())
+    z, want = c.gated_linear_fp8(x, w, wu, "relu"), c.quantize_fp8(h)
+    assert torch.equal(z.scales, want.scales) and torch.equal(z.values.view(torch.uint8), want.values.view(torch.uint8))
+
+
+def test_fp8_few_rows_nan_stays_in_its_row():
+    c = capi()
+    a = randn(12, 300, seed=1)
+    clean = c.segment_mm_fp8(c.quantize_fp8(a), weights(1, 300, 130, 3), out_dtype=F32)
+    a[5, 299] = float("nan")
+    y = c.segment_mm_fp8(c.quantize_fp8(a), weights(1, 300, 130, 3), out_dtype=F32)
+    keep = torch.arange(12, device="cuda") != 5
+    assert torch.isnan(y[5]).all() and torch.equal(y[keep], clean[keep])
+
+
 def test_mm_fp8_scale_layouts_and_views():
     c = capi()
     x, w = codes(40, 600, 1), weights(1, 600, 96, 2)

@@ -116,3 +116,13 @@ def test_changed_inputs_are_noticed():
         x.add_(1)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_codes_without_padding_behind_the_last_row_are_refused():
+    s = torch.ones(3, 1, device="cuda")
+    whole = torch.zeros(3 * 48, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn).as_strided((3, 36), (48, 1))
+    assert capi.segment_mm_fp8(capi.Fp8Rows(whole, s), capi.quantize_fp8_weight(torch.ones(36, 16, device="cuda"))).shape == (3, 16)
+    short = torch.zeros(3 * 48 - 12, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn).as_strided((3, 36), (48, 1))
+    with pytest.raises(capi.GphlError, match="padded"):
+        capi.segment_mm_fp8(capi.Fp8Rows(short, s), capi.quantize_fp8_weight(torch.ones(36, 16, device="cuda")))
