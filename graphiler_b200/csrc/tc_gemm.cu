@@ -992,6 +992,7 @@ int gemm(const GemmCall &c, const char *what, cudaStream_t stream) {
     return rc != GPHL_OK || few == 0 ? rc : join(c, a, few, stream);
   }
   if (!encode_fn()) return fail(GPHL_ERR_CUDA, "%s: cuTensorMapEncodeTiled is not available from this driver", what);
+  GPHL_CUDA(cudaSetDevice(dev));       // tensor maps are made by the driver, which wants a context: a thread's first call (of an autograd thread) finds none
   const Shape s = shape_of(c, sms);
   const bool pairs_of_b = paired(c);
   const int pairs = c.dual == DUAL_NONE ? 1 : 2;

@@ -484,6 +484,27 @@ def test_two_streams_at_once():
         assert torch.equal(g, want[i % 2])
 
 
+def test_first_call_of_a_thread():
+    """A thread that has made no CUDA call yet, its memory in the allocator's cache: as autograd's threads at the first backward pass."""
+    import threading
+    c = capi()
+    x, w = randn(300, 256, seed=1, dtype=BF16), randn(256, 512, seed=2, dtype=BF16)
+    q, qw = codes(300, 256, 3), weights(1, 256, 512, 4)
+    dh = randn(300, 512, seed=5, dtype=BF16)
+    calls = [lambda: c.gated_linear(x, w, w), lambda: c.segment_mm_fp8(q, qw), lambda: c.gated_linear_grad(dh, None, None, x, w, w)[1]]
+    want = [f() for f in calls]
+    spare = [f() for f in calls]
+    torch.cuda.synchronize()
+    del spare                                        # the threads' outputs take these blocks
+    got = []
+    for f in calls:
+        t = threading.Thread(target=lambda: got.append(f()))
+        t.start()
+        t.join()
+    torch.cuda.synchronize()
+    assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_captured_calls_keep_their_scratch_apart():
     """Two graphs whose calls need scratch (k is split), replayed in turn and with new inputs."""
     c = capi()
