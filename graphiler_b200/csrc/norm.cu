@@ -60,16 +60,11 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
   float ss = 0.f;
   // a step of r, from the inputs; stored where there is a residual
   auto take = [&](typename R::Raw t, const typename R::Raw &u, int step, float (&f)[E]) {
-    R::widen(t, f);
     if (res) {
-      float g[E];
-      R::widen(u, g);
-#pragma unroll
-      for (int j = 0; j < E; ++j) f[j] += g[j];
-      t = R::round(f);
-      R::widen(t, f);
+      t = R::add(t, u);
       if (r) R::store(r, step, lane, a.n, t);
     }
+    R::widen(t, f);
   };
   if constexpr (NV > 0) {
     typename R::Raw xs[NV], rs[NV];

@@ -87,6 +87,26 @@ template <typename T, bool SC, int LPR_ = 32> struct Row {
     }
     return x;
   }
+  // The sum rounded to T.  (The packed addition of 16-bit values rounds the exact sum once, like an addition in 32 bits and its rounding.)
+  __device__ static __forceinline__ Raw add(const Raw &x, const Raw &y) {
+    Raw z;
+    if constexpr (E == 8) {
+      using T2 = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>::type;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const T2 s = __hadd2_rn(*reinterpret_cast<const T2 *>(&x.w[j]), *reinterpret_cast<const T2 *>(&y.w[j]));
+        z.w[j] = *reinterpret_cast<const uint32_t *>(&s);
+      }
+    } else {
+      float a[E], b[E];
+      widen(x, a);
+      widen(y, b);
+#pragma unroll
+      for (int j = 0; j < E; ++j) a[j] += b[j];
+      z = round(a);
+    }
+    return z;
+  }
   __device__ static __forceinline__ void store(T *__restrict__ row, int step, int lane, int n, const Raw &x) {
     if constexpr (SC) {
 #pragma unroll
