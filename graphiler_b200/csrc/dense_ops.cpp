@@ -150,16 +150,17 @@ bool wants_grad(std::initializer_list<const Tensor *> ts) {
   return false;
 }
 
-// A captured backward pass must not reach gradients that belong to another stream: the engine would make that stream wait for the capture,
-// which ends the process.  An input's gradient belongs to the stream of the graph that it is part of: for a leaf, of any living graph.
+// A captured backward pass must not reach gradients that belong to the default stream: the engine would make that stream wait for the
+// capture, which ends the process.  An input's gradient belongs to the stream of the graph that it is part of: for a leaf, of any living graph.
+// (Other streams may join a capture: warm-up on a side stream, with its outputs kept, is fine.)
 void capturable(std::initializer_list<const Tensor *> ts, const char *what) {
   if (at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None) return;
   for (const Tensor *t : ts) {
     if (!t->defined() || !t->requires_grad()) continue;
     const auto node = t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn();
     const auto stream = node ? node->stream() : std::nullopt;
-    TORCH_CHECK(!stream || *stream == at::cuda::getCurrentCUDAStream(t->get_device()).unwrap(), what,
-                ": an input's gradients belong to a graph that was recorded on another stream than the one that is captured (drop that graph's outputs first)");
+    TORCH_CHECK(!stream || *stream != c10::cuda::getDefaultCUDAStream(t->get_device()).unwrap(), what,
+                ": an input's gradients belong to a graph that was recorded on the default stream, which a capture cannot reach (drop that graph's outputs first)");
   }
 }
 

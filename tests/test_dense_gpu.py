@@ -556,7 +556,7 @@ def test_captured_training_step():
 
 
 def test_capture_beside_a_living_graph_is_refused():
-    """An eager graph of the same leaves lives: a captured backward pass would reach its stream."""
+    """An eager graph of the same leaves, recorded on the default stream, lives: a captured backward pass would reach that stream."""
     from graphiler_b200 import capi as c, dense
     x, wg, wu, dh = gated_inputs(40, 96, 128, BF16, False)
     nw = torch.ones(96, device="cuda", dtype=BF16).requires_grad_(True)
@@ -565,9 +565,9 @@ def test_capture_beside_a_living_graph_is_refused():
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         y = x + 1
-        with pytest.raises(c.GphlError, match="another stream"):
+        with pytest.raises(c.GphlError, match="default stream"):
             dense.rms_norm(x, nw)
-        with pytest.raises(c.GphlError, match="another stream"):
+        with pytest.raises(c.GphlError, match="default stream"):
             dense.gated_linear(x, wg, wu)
         with torch.no_grad():
             h = dense.gated_linear(x, wg, wu)
@@ -583,6 +583,34 @@ def test_capture_beside_a_living_graph_is_refused():
     want = torch.autograd.grad(dense.gated_linear(dense.rms_norm(x, nw), wg, wu), (wg, nw), dh)
     assert torch.equal(dw, want[0]) and torch.equal(dn, want[1])
     del g
+
+
+@pytest.mark.filterwarnings("ignore:The AccumulateGrad node's stream")
+def test_capture_after_a_warm_up_whose_outputs_are_kept():
+    """The usual recipe: warm-up on a side stream, its last outputs still there, then the capture."""
+    from graphiler_b200 import dense
+    x, wg, wu, dh = gated_inputs(40, 96, 128, BF16, False)
+    nw = torch.ones(96, device="cuda", dtype=BF16).requires_grad_(True)
+    leaves = [nw, wg.requires_grad_(True), wu.requires_grad_(True)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            for t in leaves:
+                t.grad = None
+            y = dense.gated_linear(dense.rms_norm(x, nw), wg, wu)
+            y.backward(dh)
+        want = [t.grad for t in leaves]
+    torch.cuda.current_stream().wait_stream(s)
+    for t in leaves:
+        t.grad = None
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dense.gated_linear(dense.rms_norm(x, nw), wg, wu).backward(dh)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(t.grad, v) for t, v in zip(leaves, want))
+    del g, y
 
 
 def test_results_repeat_bit_for_bit():
