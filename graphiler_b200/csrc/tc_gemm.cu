@@ -878,8 +878,9 @@ struct Shape {
 };
 // Tile width, blocks per tile and parts of k by an estimate of the time, in microseconds: waves of tiles times steps times the measured
 // time of a step (128 bytes of k: 0.40 for a pair of blocks with 256 columns in 16 bits, 0.48 in e4m3, 0.50 for one block, less for narrower
-// tiles, which read A more often), at least the time of the operands' bytes at the rate that tiles of that width were seen to stream them, and
-// for parts their join (3, and the parts' fp32 sums written and read at 5 TB/s).  In e4m3: 2048 x 11264 -> 4096 takes 112 with k whole, 141 in
+// tiles, which read A more often, but 0.41 in e4m3, where an accumulator's way to the epilogue and back takes that long), at least the time of the
+// operands' bytes at the rate that tiles of that width, or the SMs at work, were seen to stream them (5 x 4096 -> 11264 in bf16 on 88 SMs 41.8,
+// in 3 parts on all 38.6; 64 x 4096 -> 8192 in e4m3 with 64 columns a tile 19.2, with 128 and 2 parts 16.2), and for parts their join (3, and the parts' fp32 sums written and read at 5 TB/s).  In e4m3: 2048 x 11264 -> 4096 takes 112 with k whole, 141 in
 // 2 parts; 1 x 4096 -> 8192 18.7 in 2 parts, 14.0 in 4; 1 x 16384 -> 16384 73 with 128 columns a tile, 59 with 256 and 2 parts.
 // The tensor core truncates when it adds to an fp32 accumulator: over k values of one sign a sum loses 5.4e-9 k of itself (65,536: 3.5e-4,
 // 524,288: 3.0e-3), so in 16 bits no part is longer than CHAIN (1.8e-4, below half a step of the results); the join adds with rounding.
@@ -912,12 +913,14 @@ static Shape shape_of(const GemmCall &c, int sms) {
       const int out = two ? bn / 2 : bn, units = sms / ctas;
       s.tiles_n = (c.n + out - 1) / out;
       const int64_t items = s.tiles_m * s.tiles_n * s.batch;
-      const double rate = bn == 256 ? 5.2e6 : bn == 128 ? 4.0e6 : 3.2e6;      // bytes a microsecond
-      const double step = bn == 256 ? (ctas == 1 ? 0.50 : c.fp8 ? 0.48 : 0.40) : bn == 128 ? 0.32 : 0.24;
+      const double most = bn == 256 ? 5.5e6 : bn == 128 ? 4.0e6 : 3.2e6, each = 0.052e6;      // bytes a microsecond, of all SMs and of one
+      const double step = bn == 256 ? (ctas == 1 ? 0.50 : c.fp8 ? 0.48 : 0.40) : c.fp8 ? 0.41 : bn == 128 ? 0.32 : 0.24;
+      const double finish = c.fp8 ? bn * (3.0 / 256) : 1.5;       // a tile's end (e4m3: the sums are in registers, no accumulator hides it)
       const int least = c.fp8 ? 1 : (int)std::min<int64_t>(256, (s.kt * (int64_t)ke + CHAIN - 1) / CHAIN);
       for (int p = least; p == least || (p <= 64 && p * 4 <= s.kt && items < 2 * units && items * p <= 8 * units); ++p) {
         const double waves = (double)((items * p + units - 1) / units);
-        double us = std::max(waves * ((double)s.kt / p * step + 1.5), bytes / rate);
+        const double rate = std::min(most, each * ctas * (double)std::min<int64_t>(items * p, units));
+        double us = std::max(waves * ((double)s.kt / p * step + finish), bytes / rate);
         if (p > 1) us += 3.0 + (double)p * s.batch * c.m * wide * 8.0 / 5e6;
         if (us < best_us * 0.999) best_us = us, best = s, best.splits = p;
       }
