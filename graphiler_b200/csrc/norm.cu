@@ -380,8 +380,9 @@ template <typename T, typename R> static void grad_launch(NormGradArgs a, int sm
     else rms_norm_grad_kernel<T, R, 1024><<<g.grid, g.warps * 32, g.smem, s>>>(a);
   } else if constexpr (R::LPR == 32) {
     a.wpr = 16;
-    rms_norm_grad_wide_kernel<T, R><<<(unsigned)a.m, 512, 0, s>>>(a);
+    // dw's parts first: dx may lie over dy
     rms_norm_dw_wide_kernel<T><<<dim3((unsigned)((a.n + 255) / 256), (unsigned)g.grid), 256, 0, s>>>(a);
+    rms_norm_grad_wide_kernel<T, R><<<(unsigned)a.m, 512, 0, s>>>(a);
   }
 }
 

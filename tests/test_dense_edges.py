@@ -1,0 +1,89 @@
+"""Dense operators at the edges of what is documented: results over their inputs, infinities, tails, long sums, empty products."""
+import ctypes
+
+import pytest
+import torch
+
+import dense_ref as ref
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+F8 = torch.float8_e4m3fn
+CODE = {F32: 0, BF16: 1, F16: 2}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def built():
+    from graphiler_b200 import build
+    build.build_all()
+
+
+def capi():
+    from graphiler_b200 import capi as c
+    return c
+
+
+def randn(*shape, seed=0, scale=1.0, dtype=F32):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def c_call(name, *args):
+    """An entry of the C ABI on the current stream; tensors go as addresses."""
+    c = capi()
+    args = [None if a is None else ctypes.c_void_p(a.data_ptr()) if isinstance(a, torch.Tensor) else a for a in args]
+    c._check(getattr(c.lib(), name)(*args, ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)), name)
+
+
+# ---- results over inputs, as the C ABI allows ---------------------------------------------------------------------------
+
+WIDTHS = [64, 256, 1001, 4096, 9001, 16384, 16400, 20001]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", WIDTHS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("over", ["y is x", "r is x", "r is residual", "y is x, r is residual"])
+def test_norm_over_its_inputs(n, dtype, over):
+    m = 200
+    x, res, w = randn(m, n, seed=1, dtype=dtype), randn(m, n, seed=2, dtype=dtype), randn(n, seed=3, dtype=dtype)
+    y, r, rstd = capi().rms_norm(x, w, 1e-6, residual=res, return_rstd=True)
+    a, b, got_rstd = x.clone(), res.clone(), torch.empty(m, device="cuda")
+    got_y = a if "y is x" in over else torch.empty_like(x)
+    got_r = a if "r is x" in over else b if "r is residual" in over else torch.empty_like(x)
+    c_call("gphl_rms_norm", CODE[dtype], m, n, a, b, w, CODE[dtype], 1e-6, got_y, got_r, got_rstd)
+    assert torch.equal(got_y, y) and torch.equal(got_r, r) and torch.equal(got_rstd, rstd)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", WIDTHS)
+@pytest.mark.parametrize("over", ["x", "residual"])
+def test_norm_to_codes_over_its_inputs(n, over):
+    m, pad, blocks = 70, -(-n // 16) * 16, -(-n // 128)
+    x, res, w = randn(m, n, seed=1, dtype=BF16), randn(m, n, seed=2, dtype=BF16), randn(n, seed=3, dtype=BF16)
+    q, r = capi().rms_norm_fp8(x, w, 1e-6, residual=res)
+    a, b = x.clone(), res.clone()
+    codes, scales = torch.empty(m, pad, dtype=torch.uint8, device="cuda"), torch.empty(blocks, m, device="cuda")
+    got_r = a if over == "x" else b
+    c_call("gphl_rms_norm_fp8", 1, m, n, a, b, w, 1, 1e-6, codes, pad, scales, m, got_r)
+    assert torch.equal(got_r, r) and torch.equal(scales.t(), q.scales) and torch.equal(codes[:, :n], q.values.view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", WIDTHS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("over", ["dy", "dr"])
+def test_norm_gradient_over_its_inputs(n, dtype, over):
+    """More rows than the 64 groups in which dw of wide rows is summed."""
+    m, c = 200, capi()
+    r, w, dy, dr = (randn(*s, seed=i, dtype=dtype) for i, s in enumerate([(m, n), (n,), (m, n), (m, n)]))
+    _, rstd = c.rms_norm(r, w, 1e-6, return_rstd=True)
+    dx, dw = c.rms_norm_grad(r, w, rstd, dy, dr)
+    _, rstd64, _ = ref.rms_norm(r, None, w, 1e-6)
+    want_dx, want_dw, size, size_dw = ref.rms_norm_grad(r, rstd64, w, dy, dr)
+    ref.close(dx, want_dx, ref.FP32 * size, what="dx")
+    ref.close(dw, want_dw, (ref.FP32 + m * 2.0 ** -24) * size_dw, what="dw")
+    a, b, got = dy.clone(), dr.clone(), torch.empty_like(w)
+    work = torch.empty(c.lib().gphl_rms_norm_grad_workspace_bytes(CODE[dtype], m, n), dtype=torch.uint8, device="cuda")
+    out = a if over == "dy" else b
+    c_call("gphl_rms_norm_grad", CODE[dtype], m, n, r, w, CODE[dtype], rstd, a, b, out, got, work)
+    assert torch.equal(out, dx) and torch.equal(got, dw)
