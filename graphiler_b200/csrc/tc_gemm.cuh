@@ -87,7 +87,7 @@ template <int ACT> __device__ __forceinline__ float activate(float g) {
     float e;
     return g * normal_cdf(g, e);
   }
-  return g > 0.f ? g : 0.f * g;                    // a NaN stays one
+  return g <= 0.f ? 0.f : g;                       // a NaN stays one, -inf gives 0
 }
 // dg = dh u act'(g), du = dh act(g)
 template <int ACT> __device__ __forceinline__ void gate_grads(float dh, float &g, float &u) {

@@ -87,3 +87,37 @@ def test_norm_gradient_over_its_inputs(n, dtype, over):
     out = a if over == "dy" else b
     c_call("gphl_rms_norm_grad", CODE[dtype], m, n, r, w, CODE[dtype], rstd, a, b, out, got, work)
     assert torch.equal(out, dx) and torch.equal(got, dw)
+
+
+# ---- infinities and tails of the activations ----------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("m,k", [(1, 8), (300, 8), (2, 4096)])
+def test_relu_of_infinities(m, k, dtype):
+    """g of -inf gives 0, of +inf +inf, of NaN NaN; with gradients from above, that of u is 0 where act is (k = 4096: k is split)."""
+    c = capi()
+    x, wg, wu = torch.ones(m, k, dtype=dtype, device="cuda"), torch.ones(k, 40, dtype=dtype, device="cuda"), torch.ones(k, 40, dtype=dtype, device="cuda")
+    wg[0, 3], wg[0, 5], wg[0, 7], wg[0, 9] = float("-inf"), float("inf"), float("nan"), -2.0 * k
+    h, g, u = c.gated_linear(x, wg, wu, "relu", return_projections=True)
+    want = torch.full((40,), float(k) * k, device="cuda")
+    want[3], want[5], want[7], want[9] = 0, float("inf"), float("nan"), 0
+    assert torch.equal(torch.nan_to_num(h, nan=-7.0), torch.nan_to_num(want.to(dtype).expand(m, 40), nan=-7.0))
+    dh = torch.ones(m, 40, dtype=dtype, device="cuda")
+    for kept in ((g, u), (None, None)):
+        _, dwg, dwu = c.gated_linear_grad(dh, *kept, x, wg, wu, "relu", want_dx=False)
+        for col in (3, 9):
+            assert (dwg[:, col] == 0).all() and (dwu[:, col] == 0).all()
+        assert torch.isinf(dwu[:, 5]).all() and torch.isnan(dwu[:, 7]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 8, 40, 300])
+def test_relu_of_infinities_in_8_bits(m):
+    """Scales whose product is beyond fp32: g = -inf, h = 0, as a value and as codes."""
+    c = capi()
+    row = lambda v, s: c.Fp8Rows(torch.full((m, 128), v, device="cuda").to(F8), torch.full((m, 1), s, device="cuda"))
+    weight = lambda v, s: c.Fp8Weight(torch.full((1, 32, 128), v, device="cuda").to(F8), torch.full((1, 1, 1), s, device="cuda"))
+    x, wg, wu = row(1.0, 2.0 ** 100), weight(-1.0, 2.0 ** 100), weight(1.0, 2.0 ** -100)
+    assert (c.gated_linear_fp8(x, wg, wu, "relu", out_dtype=F32) == 0).all()
+    assert (c.dequantize_fp8(c.gated_linear_fp8(x, wg, wu, "relu")) == 0).all()
