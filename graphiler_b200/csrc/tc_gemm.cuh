@@ -71,14 +71,16 @@ __device__ __forceinline__ float rcp_fast(float x) {
 }
 constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float sigmoid_fast(float g) { return rcp_fast(1.f + exp2_fast(-LOG2E * g)); }
-// Phi(g), and exp(-g^2 / 2) by the way: Phi(-x) = P(t) exp(-x^2 / 2) / 2, t = 1 / (1 + 0.3275911 x / sqrt 2), the rational
-// approximation 7.1.26 of Abramowitz and Stegun's Handbook of Mathematical Functions for erf (absolute error 1.5e-7); the tail keeps
-// its leading digits, which 1 + erf does not.
+// Phi(g), and e = exp(-g^2 / 2) by the way.  The tail is Phi(-x) = e P(t) with t = 1 / (1 + 0.3 x): P is a polynomial without a constant term
+// whose relative error over 0 <= x <= 14 was made as small as possible (1.5e-7 exactly evaluated, 4.8e-7 in fp32), so that Phi keeps its leading
+// digits down to where e leaves fp32 (g = -13.2).  Farther out e's own argument bounds it: g^2 / 2 is off by 1.5 * 2^-24 of itself (g = -8: 3e-6).
 __device__ __forceinline__ float normal_cdf(float g, float &e) {
-  const float t = rcp_fast(fmaf(0.3275911f * 0.70710678118654752f, fabsf(g), 1.f));
+  const float t = rcp_fast(fmaf(0.3f, fabsf(g), 1.f));
   e = exp2_fast(-0.5f * LOG2E * g * g);
-  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  const float tail = 0.5f * p * e;
+  float p = fmaf(t, 0.035674773f, -0.15720308f);
+  p = fmaf(t, p, 0.2063535f), p = fmaf(t, p, -0.05368364f), p = fmaf(t, p, 0.12856163f);
+  p = fmaf(t, p, 0.09991349f), p = fmaf(t, p, 0.12075396f), p = fmaf(t, p, 0.1196293f);
+  const float tail = t * p * e;
   return g < 0.f ? tail : 1.f - tail;
 }
 template <int ACT> __device__ __forceinline__ float activate(float g) {
@@ -104,8 +106,8 @@ template <int ACT> __device__ __forceinline__ void gate_grads(float dh, float &g
   }
   g = dh * u * d, u = dh * h;
 }
-// Two neighbouring elements at once: h = act(g) u, and the pair dg, du into g, u.  silu in packed arithmetic (one instruction for both
-// elements but for exponential and reciprocal).
+// Two neighbouring elements at once: h = act(g) u, and the pair dg, du into g, u.  silu and gelu in packed arithmetic (one instruction for both
+// elements but for exponential and reciprocal; gelu, 300,000 x 256 -> 1024 in bf16: 430 to 450 us forward, 482 an element at a time).
 __device__ __forceinline__ uint64_t both(float v) { return pack2(v, v); }
 __device__ __forceinline__ uint64_t sigmoid2(uint64_t g) {
   float a, b;
@@ -113,10 +115,29 @@ __device__ __forceinline__ uint64_t sigmoid2(uint64_t g) {
   unpack2(fadd2(pack2(exp2_fast(a), exp2_fast(b)), both(1.f)), a, b);
   return pack2(rcp_fast(a), rcp_fast(b));
 }
+__device__ __forceinline__ uint64_t normal_cdf2(uint64_t g, uint64_t &e) {
+  float a, b, g0, g1, t0, t1;
+  unpack2(ffma2(both(0.3f), g & 0x7fffffff7fffffffull, both(1.f)), a, b);
+  const uint64_t t = pack2(rcp_fast(a), rcp_fast(b));
+  unpack2(fmul2(fmul2(both(-0.5f * LOG2E), g), g), a, b);
+  e = pack2(exp2_fast(a), exp2_fast(b));
+  uint64_t p = ffma2(t, both(0.035674773f), both(-0.15720308f));
+  p = ffma2(t, p, both(0.2063535f)), p = ffma2(t, p, both(-0.05368364f)), p = ffma2(t, p, both(0.12856163f));
+  p = ffma2(t, p, both(0.09991349f)), p = ffma2(t, p, both(0.12075396f)), p = ffma2(t, p, both(0.1196293f));
+  const uint64_t tail = fmul2(fmul2(t, p), e);
+  unpack2(tail, t0, t1);
+  unpack2(fsub2(both(1.f), tail), a, b);
+  unpack2(g, g0, g1);
+  return pack2(g0 < 0.f ? t0 : a, g1 < 0.f ? t1 : b);
+}
 template <int ACT> __device__ __forceinline__ void gate2(float &g0, float &g1, float u0, float u1) {
   if constexpr (ACT == ACT_SILU) {
     const uint64_t g = pack2(g0, g1);
     unpack2(fmul2(fmul2(g, sigmoid2(g)), pack2(u0, u1)), g0, g1);
+  } else if constexpr (ACT == ACT_GELU) {
+    uint64_t e;
+    const uint64_t g = pack2(g0, g1);
+    unpack2(fmul2(fmul2(g, normal_cdf2(g, e)), pack2(u0, u1)), g0, g1);
   } else {
     g0 = activate<ACT>(g0) * u0, g1 = activate<ACT>(g1) * u1;
   }
@@ -125,6 +146,12 @@ template <int ACT> __device__ __forceinline__ void gate_grads2(float dh0, float 
   if constexpr (ACT == ACT_SILU) {
     const uint64_t dh = pack2(dh0, dh1), g = pack2(g0, g1), s = sigmoid2(g), h = fmul2(g, s);
     const uint64_t d = ffma2(h, fsub2(both(1.f), s), s);
+    unpack2(fmul2(fmul2(dh, pack2(u0, u1)), d), g0, g1);
+    unpack2(fmul2(dh, h), u0, u1);
+  } else if constexpr (ACT == ACT_GELU) {
+    uint64_t e;
+    const uint64_t dh = pack2(dh0, dh1), g = pack2(g0, g1), c = normal_cdf2(g, e), h = fmul2(g, c);
+    const uint64_t d = ffma2(fmul2(both(0.39894228040143268f), g), e, c);
     unpack2(fmul2(fmul2(dh, pack2(u0, u1)), d), g0, g1);
     unpack2(fmul2(dh, h), u0, u1);
   } else {

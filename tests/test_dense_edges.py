@@ -121,3 +121,63 @@ def test_relu_of_infinities_in_8_bits(m):
     x, wg, wu = row(1.0, 2.0 ** 100), weight(-1.0, 2.0 ** 100), weight(1.0, 2.0 ** -100)
     assert (c.gated_linear_fp8(x, wg, wu, "relu", out_dtype=F32) == 0).all()
     assert (c.dequantize_fp8(c.gated_linear_fp8(x, wg, wu, "relu")) == 0).all()
+
+
+def gelu_bound(g):
+    """Relative error of Phi(g): fp32 arithmetic of a fit that is right to 2^-22 and two approximate instructions (2^-19 in all), and the exponent
+    g^2 / 2, two products and a rounded constant: 1.5 * 2^-24 of it each way and 2^-23 of room."""
+    return 2.0 ** -19 + g.square() * 2.0 ** -23
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 40])
+def test_gelu_keeps_its_leading_digits_8_bits(m):
+    """g over the e4m3 values of [-12, 12] with u = 1, results in 32 bits: relative to the value itself, also where it is small."""
+    c = capi()
+    codes = torch.arange(256, dtype=torch.int32, device="cuda").to(torch.uint8).view(F8).float()
+    g = codes[codes.abs() <= 12].sort().values
+    n = g.numel()
+    wg, wu = torch.zeros(1, n, 16, device="cuda"), torch.zeros(1, n, 16, device="cuda")
+    wg[0, :, 0], wu[0, :, 1] = g, 1.0
+    x = torch.zeros(m, 16, device="cuda")
+    x[:, :2] = 1.0
+    one = torch.ones(m, 1, device="cuda"), torch.ones(1, -(-n // 128), 1, device="cuda")
+    h = c.gated_linear_fp8(c.Fp8Rows(x.to(F8), one[0]), c.Fp8Weight(wg.to(F8), one[1]), c.Fp8Weight(wu.to(F8), one[1]), "gelu", out_dtype=F32)
+    want = g.double() * torch.exp(torch.special.log_ndtr(g.double()))
+    ref.close(h, want.expand(m, n), (gelu_bound(g.double()) * want.abs()).expand(m, n), what="gelu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("m", [1, 300])
+def test_activations_of_large_values(act, m):
+    """+inf stays, NaN stays, and far below 0 nothing is left."""
+    x, wg, wu = (torch.ones(*s, dtype=BF16, device="cuda") for s in ((m, 8), (8, 40), (8, 40)))
+    wg[0, 3], wg[0, 5], wg[0, 7], wg[0, 9] = float("inf"), float("nan"), 1e30, -1e30
+    h = capi().gated_linear(x, wg, wu, act).float()
+    assert (h[:, 3] == float("inf")).all() and torch.isnan(h[:, 5]).all() and (h[:, 9] == 0).all()
+    ref.close(h[:, 7].bfloat16(), (8 * wg[0, 7].double()).expand(m), (ref.FP32 * 8e30 * torch.ones(m, dtype=torch.float64, device="cuda")))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_gelu_keeps_its_leading_digits_with_gradients(dtype):
+    """One row: the weights' gradients are dg and du themselves.  u = 2^10, so that fp16 holds the tail."""
+    c = capi()
+    g = torch.arange(-96, 49, device="cuda") / 16.0                   # -6 .. 3, exact in both types
+    n, size = g.numel(), 1024.0
+    wg, wu = torch.zeros(8, n, device="cuda"), torch.zeros(8, n, device="cuda")
+    wg[0], wu[1] = g, size
+    x, wg, wu, dh = torch.ones(1, 8, device="cuda").to(dtype), wg.to(dtype), wu.to(dtype), torch.full((1, n), 4.0, dtype=dtype, device="cuda")
+    h, gg, uu = c.gated_linear(x, wg, wu, "gelu", return_projections=True)
+    assert torch.equal(gg[0, :n], g) and (uu[0, :n] == size).all()
+    g = g.double()
+    phi, dens = torch.special.ndtr(g), torch.exp(-g * g / 2) / (2 * torch.pi) ** 0.5
+    act, err = g * phi, gelu_bound(g) * (g * phi).abs()
+    ref.close(h, (size * act)[None], (size * err)[None], what="h")
+    # act' = Phi + g phi: the second term's exponential is off by as much, and the sum cancels near g = -0.75
+    dact, derr = phi + g * dens, gelu_bound(g) * (phi + g.abs() * dens)
+    for kept in ((gg, uu), (None, None)):
+        _, dwg, dwu = c.gated_linear_grad(dh, *kept, x, wg, wu, "gelu", want_dx=False)
+        ref.close(dwu[0], 4 * act, 4 * err, what="du")
+        ref.close(dwg[0], 4 * size * dact, 4 * size * derr, what="dg")
