@@ -179,9 +179,10 @@ def prepare_feed_forward_fp8(p: Dict[str, torch.Tensor]):
 
 
 def feed_forward_layer_fp8(h, q, residual=None, eps: float = 1e-6, activation: str = "silu"):
-    """``feed_forward_layer`` for serving, in 8 bits: three kernels, the rows between them e4m3 with a scale per 128 values; the sum
-    with r is in the rows' type.  ``q``: ``prepare_feed_forward_fp8``."""
+    """``feed_forward_layer`` for serving, in 8 bits, on (m, d) rows of any of the three types: norm, gated product and product back, the rows between them
+    e4m3 with a scale per 128 values; the product is rounded to the rows' type and r added to it there.  No gradients are recorded,
+    not even of r.  ``q``: ``prepare_feed_forward_fp8``."""
     n = capi.rms_norm_fp8(h, q["norm_weight"], eps, residual=residual)
-    n, r = (n, h) if residual is None else n
+    n, r = (n, h.detach()) if residual is None else n
     g = capi.gated_linear_fp8(n, q["gate_weight"], q["up_weight"], activation)
     return capi.segment_mm_fp8(g, q["down_weight"], out_dtype=h.dtype).add_(r)

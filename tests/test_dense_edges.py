@@ -181,3 +181,24 @@ def test_gelu_keeps_its_leading_digits_with_gradients(dtype):
         _, dwg, dwu = c.gated_linear_grad(dh, *kept, x, wg, wu, "gelu", want_dx=False)
         ref.close(dwu[0], 4 * act, 4 * err, what="du")
         ref.close(dwg[0], 4 * size * dact, 4 * size * derr, what="dg")
+
+
+# ---- the layers -----------------------------------------------------------------------------------------------------------
+
+def ff_params(d, f, dtype=BF16):
+    return {"norm_weight": 1 + 0.2 * randn(d, seed=7).to(dtype), "gate_weight": randn(d, f, seed=8, scale=d ** -0.5, dtype=dtype),
+            "up_weight": randn(d, f, seed=9, scale=d ** -0.5, dtype=dtype), "down_weight": randn(f, d, seed=10, scale=f ** -0.5, dtype=dtype)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("with_res", [False, True])
+def test_the_serving_layer_records_no_gradients(with_res):
+    """Not a part of them either: the sum with the input would pass its own on and nothing of the rest."""
+    from graphiler_b200 import layers
+    q = layers.prepare_feed_forward_fp8(ff_params(96, 200))
+    h, res = randn(50, 96, seed=1, dtype=BF16), randn(50, 96, seed=2, dtype=BF16) if with_res else None
+    want = layers.feed_forward_layer_fp8(h, q, residual=res)
+    kept = h.clone()
+    h.requires_grad_(True)
+    got = layers.feed_forward_layer_fp8(h, q, residual=None if res is None else res.requires_grad_(True))
+    assert not got.requires_grad and torch.equal(got, want) and torch.equal(h, kept)
