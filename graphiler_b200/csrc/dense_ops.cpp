@@ -279,7 +279,6 @@ Tensor segment_mm_fp8(const Tensor &q, const Tensor &s, const Tensor &wq, const 
   const int dt = dtype_of(type, "segment_mm_fp8: the output");
   c10::cuda::CUDAGuard guard(q.device());
   Tensor y = out ? *out : plain(q, type, {m, n});
-  if (k == 0 && !pointer.defined()) return y.zero_();
   Tensor work = scratch(gphl_segment_mm_fp8_workspace_bytes(t, pointer.defined(), m, k, n), q);
   check_rc(gphl_segment_mm_fp8(t, static_cast<const int32_t *>(ptr(pointer)), m, k, n, ptr(q), xrow, static_cast<const float *>(ptr(s)), s.stride(0),
                                s.stride(1), ptr(wq), wrow, static_cast<const float *>(ptr(ws)), dt, mut(y), mut(work), stream_of(q)),

@@ -225,8 +225,7 @@ extern "C" int gphl_segment_mm_fp8(int64_t n_types, const int32_t *type_pointer,
   GPHL_REQUIRE(known(out_dtype), "segment_mm_fp8: unknown type %d", out_dtype);
   GPHL_REQUIRE(type_pointer || n_types == 1, "segment_mm_fp8: several types need a type pointer");
   if (m == 0 || n == 0 || n_types == 0) return GPHL_OK;
-  GPHL_REQUIRE(k > 0, "segment_mm_fp8: the inner dimension is empty");
-  GPHL_REQUIRE(x && x_scales && w && w_scales && y, "null pointer argument");
+  GPHL_REQUIRE(y && (k == 0 || (x && x_scales && w && w_scales)), "null pointer argument");
   GPHL_REQUIRE(x_stride >= k && w_stride >= k, "segment_mm_fp8: code rows are shorter than k");
   GemmCall c;
   c.fp8 = true, c.m = m, c.n = n, c.k = k, c.types = n_types, c.ptr = type_pointer;

@@ -988,6 +988,7 @@ int gemm(const GemmCall &c, const char *what, cudaStream_t stream) {
   GPHL_CUDA(cudaGetDevice(&dev));
   GPHL_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   GemmArgs a = finish_args(c);
+  if (c.k == 0) return join(c, a, 0, stream);            // no parts: sums of nothing
   const int few = few_rows_parts(c);
   if (few >= 0) {
     GPHL_REQUIRE(few == 0 || (a.part && aligned16(a.part)), "%s: the workspace is missing or not 16-byte aligned", what);

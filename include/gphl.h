@@ -334,8 +334,8 @@ int gphl_dequantize_fp8(int32_t dtype, int64_t m, int64_t n, const void *q, int6
 int gphl_pad_rows_16(int64_t m, int64_t n, const void *x, void *y, void *stream);
 
 /* Typed product of codes: y[i, :] = x[i, :] @ w[t]^T for the rows i of type t, type_pointer (n_types + 1) int32 as in segment_mm or
- * NULL (one type, all rows).  Sums of a block of 128 are scaled and added in fp32.  y (m, n) row-major in out_dtype; rows of no type
- * are left as they are.  `workspace`: gphl_segment_mm_fp8_workspace_bytes. */
+ * NULL (one type, all rows).  Sums of a block of 128 are scaled and added in fp32.  y (m, n) row-major in out_dtype (k == 0: zeros); rows of no
+ * type are left as they are.  `workspace`: gphl_segment_mm_fp8_workspace_bytes. */
 int64_t gphl_segment_mm_fp8_workspace_bytes(int64_t n_types, int32_t typed, int64_t m, int64_t k, int64_t n);
 int gphl_segment_mm_fp8(int64_t n_types, const int32_t *type_pointer, int64_t m, int64_t k, int64_t n, const void *x, int64_t x_stride,
                         const float *x_scales, int64_t scale_row_stride, int64_t scale_block_stride, const void *w, int64_t w_stride,

@@ -202,3 +202,20 @@ def test_the_serving_layer_records_no_gradients(with_res):
     h.requires_grad_(True)
     got = layers.feed_forward_layer_fp8(h, q, residual=None if res is None else res.requires_grad_(True))
     assert not got.requires_grad and torch.equal(got, want) and torch.equal(h, kept)
+
+
+# ---- the typed product's arguments ------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_mm_fp8_of_an_empty_inner_dimension(dtype):
+    """Sums of nothing: zeros in the rows of any type, with a pointer as without; rows of no type stay."""
+    c = capi()
+    x = c.Fp8Rows(torch.empty(300, 0, dtype=torch.uint8, device="cuda").view(F8), torch.empty(300, 0, device="cuda"))
+    w = lambda t: c.Fp8Weight(torch.empty(t, 40, 0, dtype=torch.uint8, device="cuda").view(F8), torch.empty(t, 1, 0, device="cuda"))
+    assert (c.segment_mm_fp8(x, w(1), out_dtype=dtype) == 0).all()
+    out = torch.full((300, 40), 7.0, dtype=dtype, device="cuda")
+    y = c.segment_mm_fp8(x, w(3), torch.tensor([5, 40, 40, 290], dtype=torch.int32, device="cuda"), out=out)
+    assert y is out and (out[:5] == 7).all() and (out[5:290] == 0).all() and (out[290:] == 7).all()
+    y = c.segment_mm_fp8(x, w(3), torch.tensor([0, 40, 40, 300], dtype=torch.int32, device="cuda"), out_dtype=dtype)
+    assert y.dtype == dtype and (y == 0).all()
