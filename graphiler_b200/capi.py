@@ -650,7 +650,7 @@ def dequantize_fp8(q: Fp8Rows, dtype=torch.float32):
 def segment_mm_fp8(x: Fp8Rows, w: Fp8Weight, type_pointer=None, out_dtype=torch.bfloat16, out=None):
     """``segment_mm`` on rows and weights in 8 bits: y[p_t:p_{t+1}] = x[p_t:p_{t+1}] @ w[t], blocks of 128 scaled and summed in float32.
     ``type_pointer`` (types + 1) int32, or None with one type for all rows.  Rows that no type covers are left as they are (of a
-    new ``out``: undefined)."""
+    new ``out``: undefined).  ``out`` sets the type of the result; no gradients are recorded, and one that wants them is refused."""
     return _call("segment_mm_fp8", x.values, x.scales, w.values, w.scales, type_pointer, out_dtype, out)
 
 

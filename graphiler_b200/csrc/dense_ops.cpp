@@ -274,11 +274,13 @@ Tensor segment_mm_fp8(const Tensor &q, const Tensor &s, const Tensor &wq, const 
               "segment_mm_fp8: the type pointer must hold types + 1 int32 values");
   if (out) {
     TORCH_CHECK(out->dim() == 2 && out->size(0) == m && out->size(1) == n, "segment_mm_fp8: out must be (m, n)");
+    TORCH_CHECK(!at::GradMode::is_enabled() || !out->requires_grad(), "segment_mm_fp8: out wants gradients, and none are recorded");
     type = out->scalar_type();
   }
   const int dt = dtype_of(type, "segment_mm_fp8: the output");
   c10::cuda::CUDAGuard guard(q.device());
   Tensor y = out ? *out : plain(q, type, {m, n});
+  if (out && !y.is_inference()) torch::autograd::impl::bump_version(y);      // what autograd kept of it is noticed to have changed
   Tensor work = scratch(gphl_segment_mm_fp8_workspace_bytes(t, pointer.defined(), m, k, n), q);
   check_rc(gphl_segment_mm_fp8(t, static_cast<const int32_t *>(ptr(pointer)), m, k, n, ptr(q), xrow, static_cast<const float *>(ptr(s)), s.stride(0),
                                s.stride(1), ptr(wq), wrow, static_cast<const float *>(ptr(ws)), dt, mut(y), mut(work), stream_of(q)),
@@ -464,7 +466,8 @@ TORCH_LIBRARY_FRAGMENT(my_ops, m) {
   m.def("quantize_fp8(Tensor x) -> (Tensor, Tensor)", &quantize_fp8);
   m.def("quantize_fp8_weight(Tensor w) -> (Tensor, Tensor)", &quantize_fp8_weight);
   m.def("dequantize_fp8(Tensor q, Tensor scales, ScalarType dtype) -> Tensor", &dequantize_fp8);
-  m.def("segment_mm_fp8(Tensor q, Tensor scales, Tensor w, Tensor w_scales, Tensor? type_pointer, ScalarType dtype, Tensor? out) -> Tensor", &segment_mm_fp8);
+  m.def("segment_mm_fp8(Tensor q, Tensor scales, Tensor w, Tensor w_scales, Tensor? type_pointer, ScalarType dtype, Tensor(a!)? out) -> Tensor(a!)",
+        &segment_mm_fp8);
   m.def("gated_linear(Tensor x, Tensor w_gate, Tensor w_up, str activation) -> Tensor", &gated_linear);
   m.def("gated_linear_rows(Tensor x, Tensor w_gate, Tensor w_up, str activation, bool return_projections) -> Tensor[]", &gated_rows);
   m.def("gated_linear_grad(Tensor dh, Tensor? g, Tensor? u, Tensor x, Tensor w_gate, Tensor w_up, str activation, bool want_dx, bool want_dw) -> Tensor[]",

@@ -219,3 +219,30 @@ def test_mm_fp8_of_an_empty_inner_dimension(dtype):
     assert y is out and (out[:5] == 7).all() and (out[5:290] == 0).all() and (out[290:] == 7).all()
     y = c.segment_mm_fp8(x, w(3), torch.tensor([0, 40, 40, 300], dtype=torch.int32, device="cuda"), out_dtype=dtype)
     assert y.dtype == dtype and (y == 0).all()
+
+
+def test_mm_fp8_says_that_it_writes_out():
+    """The registration's schema, by which graph passes keep the write in its place."""
+    capi()._op("segment_mm_fp8")
+    args = {a.name: a for a in torch.ops.my_ops.segment_mm_fp8.default._schema.arguments}
+    assert "out" in args and args["out"].alias_info is not None and args["out"].alias_info.is_write
+    assert not any(a.alias_info for n, a in args.items() if n != "out")
+
+
+@pytest.mark.gpu
+def test_mm_fp8_counts_its_write():
+    """What autograd kept of `out` is known to have changed."""
+    c = capi()
+    x, w = c.quantize_fp8(randn(4, 64, seed=1)), c.quantize_fp8_weight(randn(64, 32, seed=2))
+    out = torch.ones(4, 32, device="cuda")
+    a = torch.ones(4, 32, device="cuda", requires_grad=True)
+    loss = (a * out).sum()
+    assert c.segment_mm_fp8(x, w, out=out) is out and out._version == 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with pytest.raises(c.GphlError, match="gradients"):
+        c.segment_mm_fp8(x, w, out=torch.ones(4, 32, device="cuda", requires_grad=True))
+    with torch.no_grad():
+        c.segment_mm_fp8(x, w, out=torch.ones(4, 32, device="cuda", requires_grad=True))
+    with torch.inference_mode():
+        assert torch.equal(c.segment_mm_fp8(x, w, out=torch.ones(4, 32, device="cuda")), out)
