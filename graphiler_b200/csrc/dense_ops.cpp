@@ -143,6 +143,11 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
   }
 };
 
+// A tangent would be dropped without a word where nothing else wants gradients.
+void no_tangents(std::initializer_list<const Tensor *> ts, const char *what) {
+  for (const Tensor *t : ts) TORCH_CHECK(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), what, ": no derivatives in forward mode");
+}
+
 bool wants_grad(std::initializer_list<const Tensor *> ts) {
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor *t : ts)
@@ -169,6 +174,7 @@ std::vector<Tensor> rms_norm(const Tensor &x, const Tensor &w, double eps, const
   TORCH_CHECK(x.dim() >= 1 && w.dim() == 1 && x.size(-1) == w.size(0), "rms_norm needs rows (..., n) and a weight of n values");
   TORCH_CHECK(!res.defined() || res.sizes() == x.sizes(), "rms_norm: the residual must have the rows' shape and type");
   on_device({&x, &w, &res});
+  no_tangents({&x, &w, &res}, "rms_norm");
   const Tensor wc = w.contiguous();
   if (wants_grad({&x, &w, &res})) {
     capturable({&x, &w, &res}, "rms_norm");
@@ -415,6 +421,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
 Tensor gated_linear(const Tensor &x, const Tensor &wg, const Tensor &wu, c10::string_view act) {
   TORCH_CHECK(x.dim() >= 1 && wg.dim() == 2 && x.size(-1) == wg.size(0), "gated_linear needs rows (..., k) and two weights (k, f)");
   on_device({&x, &wg, &wu});
+  no_tangents({&x, &wg, &wu}, "gated_linear");
   if (wants_grad({&x, &wg, &wu})) {
     capturable({&x, &wg, &wu}, "gated_linear");
     return GatedLinear::apply(x, wg, wu, std::string(act));

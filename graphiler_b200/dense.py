@@ -3,7 +3,7 @@ the gated feed-forward, each one autograd node over the library's kernels (csrc/
 
 The reference runs its models forward only (python/graphiler/utils/bench.py:10-49) and has no counterpart of these operators; they
 stand next to the dense projection (``layers.project``) that a graph transformer's layer applies to the node rows
-(examples/HGT/HGT.py:28-60).  Leading dimensions are flattened to rows; first derivatives only.  While a CUDA graph is captured, inputs
+(examples/HGT/HGT.py:28-60).  Leading dimensions are flattened to rows; first derivatives only, in reverse mode.  While a CUDA graph is captured, inputs
 whose gradients belong to the default stream (an eager graph of the same leaves, recorded there, still lives) are refused.
 """
 from __future__ import annotations

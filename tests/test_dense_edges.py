@@ -246,3 +246,24 @@ def test_mm_fp8_counts_its_write():
         c.segment_mm_fp8(x, w, out=torch.ones(4, 32, device="cuda", requires_grad=True))
     with torch.inference_mode():
         assert torch.equal(c.segment_mm_fp8(x, w, out=torch.ones(4, 32, device="cuda")), out)
+
+
+# ---- derivatives that there are not ------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("requires_grad", [False, True])
+def test_forward_mode_is_refused(requires_grad):
+    """A tangent is not dropped without a word."""
+    from graphiler_b200 import dense
+    from torch.autograd import forward_ad as fw
+    args = [randn(4, 64, seed=1, dtype=BF16), randn(64, seed=2, dtype=BF16), randn(4, 64, seed=3, dtype=BF16), randn(64, 32, seed=4, dtype=BF16),
+            randn(64, 32, seed=5, dtype=BF16)]
+    with fw.dual_level():
+        for i in range(5):
+            x, w, res, wg, wu = (fw.make_dual(a.clone().requires_grad_(requires_grad), torch.ones_like(a)) if i == j else a for j, a in enumerate(args))
+            if i < 3:
+                with pytest.raises(capi().GphlError, match="forward"):
+                    dense.rms_norm(x, w, residual=res)
+            if i in (0, 3, 4):
+                with pytest.raises(capi().GphlError, match="forward"):
+                    dense.gated_linear(x, wg, wu)
