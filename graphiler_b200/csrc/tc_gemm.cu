@@ -758,7 +758,9 @@ __global__ void __launch_bounds__(gemm_threads(EPI_WARPS, FP8), 1) gemm_kernel(c
 
 // ---- joining the parts of a split k ------------------------------------------------------------------------------------------------
 
-// A warp per (row, 128 columns), 4 neighbouring columns a lane; the parts are added in order.
+// A warp per (row, 128 columns), 4 neighbouring columns a lane; the parts are added in order, in groups, so that a sum over very many rows (3052
+// parts for 100 million) rounds a running sum about as often as a group is long and groups are many.
+constexpr int JOIN_GROUP = 64;
 template <int MODE> __global__ void __launch_bounds__(256) gemm_join_kernel(const GemmArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t blocks = (a.n + 127) / 128, item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -769,14 +771,19 @@ template <int MODE> __global__ void __launch_bounds__(256) gemm_join_kernel(cons
   if (a.ptr && (row < __ldg(a.ptr) || row >= __ldg(a.ptr + a.types))) return;      // a row of no type
   float4 g = make_float4(0, 0, 0, 0), u = g;
   if (c0 < a.n) {
-    for (int s = 0; s < a.splits; ++s) {
-      const float *p = a.part + ((int64_t)(s * a.batch + b) * a.m + row) * a.ld_part + c0;
-      const float4 v = *reinterpret_cast<const float4 *>(p);
-      g.x += v.x, g.y += v.y, g.z += v.z, g.w += v.w;
-      if (MODE != LINEAR) {
-        const float4 t = *reinterpret_cast<const float4 *>(p + a.part_u);
-        u.x += t.x, u.y += t.y, u.z += t.z, u.w += t.w;
+    for (int s0 = 0; s0 < a.splits; s0 += JOIN_GROUP) {
+      float4 pg = make_float4(0, 0, 0, 0), pu = pg;
+      for (int s = s0; s < min(s0 + JOIN_GROUP, a.splits); ++s) {
+        const float *p = a.part + ((int64_t)(s * a.batch + b) * a.m + row) * a.ld_part + c0;
+        const float4 v = *reinterpret_cast<const float4 *>(p);
+        pg.x += v.x, pg.y += v.y, pg.z += v.z, pg.w += v.w;
+        if (MODE != LINEAR) {
+          const float4 t = *reinterpret_cast<const float4 *>(p + a.part_u);
+          pu.x += t.x, pu.y += t.y, pu.z += t.z, pu.w += t.w;
+        }
       }
+      g.x += pg.x, g.y += pg.y, g.z += pg.z, g.w += pg.w;
+      u.x += pu.x, u.y += pu.y, u.z += pu.z, u.w += pu.w;
     }
   }
   float o[4] = {g.x, g.y, g.z, g.w};
@@ -883,7 +890,8 @@ struct Shape {
 // in 3 parts on all 38.6; 64 x 4096 -> 8192 in e4m3 with 64 columns a tile 19.2, with 128 and 2 parts 16.2), and for parts their join (3, and the parts' fp32 sums written and read at 5 TB/s).  In e4m3: 2048 x 11264 -> 4096 takes 112 with k whole, 141 in
 // 2 parts; 1 x 4096 -> 8192 18.7 in 2 parts, 14.0 in 4; 1 x 16384 -> 16384 73 with 128 columns a tile, 59 with 256 and 2 parts.
 // The tensor core truncates when it adds to an fp32 accumulator: over k values of one sign a sum loses 5.4e-9 k of itself (65,536: 3.5e-4,
-// 524,288: 3.0e-3), so in 16 bits no part is longer than CHAIN (1.8e-4, below half a step of the results); the join adds with rounding.
+// 524,288: 3.0e-3), so in 16 bits no part is longer than CHAIN (1.8e-4, below half a step of the results), however many parts that makes (both
+// weights' gradients over m rows: m k f / 4096 bytes of parts, at most k / 16384 of the operands' own); the join adds with rounding.
 constexpr int64_t CHAIN = 32768;
 static bool paired(const GemmCall &c) { return c.dual == DUAL_GATED || c.dual == DUAL_GATED_GRAD; }
 static int sm_count() {
@@ -916,7 +924,7 @@ static Shape shape_of(const GemmCall &c, int sms) {
       const double most = bn == 256 ? 5.5e6 : bn == 128 ? 4.0e6 : 3.2e6, each = 0.052e6;      // bytes a microsecond, of all SMs and of one
       const double step = bn == 256 ? (ctas == 1 ? 0.50 : c.fp8 ? 0.48 : 0.40) : c.fp8 ? 0.41 : bn == 128 ? 0.32 : 0.24;
       const double finish = c.fp8 ? bn * (3.0 / 256) : 1.5;       // a tile's end (e4m3: the sums are in registers, no accumulator hides it)
-      const int least = c.fp8 ? 1 : (int)std::min<int64_t>(256, (s.kt * (int64_t)ke + CHAIN - 1) / CHAIN);
+      const int least = c.fp8 ? 1 : (int)((s.kt * (int64_t)ke + CHAIN - 1) / CHAIN);
       for (int p = least; p == least || (p <= 64 && p * 4 <= s.kt && items < 2 * units && items * p <= 8 * units); ++p) {
         const double waves = (double)((items * p + units - 1) / units);
         const double rate = std::min(most, each * ctas * (double)std::min<int64_t>(items * p, units));

@@ -267,3 +267,34 @@ def test_forward_mode_is_refused(requires_grad):
             if i in (0, 3, 4):
                 with pytest.raises(capi().GphlError, match="forward"):
                     dense.gated_linear(x, wg, wu)
+
+
+# ---- long sums ----------------------------------------------------------------------------------------------------------------
+
+CHAIN = 32768            # values of k that one tensor-core sum may gather
+
+
+@pytest.mark.parametrize("m", [8192, 300_000, 8_388_608, 8_500_000, 100_000_000, 2_000_000_000])
+def test_gated_weight_gradients_have_room_for_all_parts(m):
+    """dW sums over the rows in parts of at most CHAIN, whose fp32 sums lie in the workspace behind dg and du."""
+    k, f = 64, 72
+    room = capi().lib().gphl_gated_grad_workspace_bytes(m, k, f) - 2 * -(-m * f * 2 // 256) * 256
+    parts = -(-m // CHAIN)
+    assert parts == 1 or room >= parts * 2 * k * f * 4
+
+
+@pytest.mark.gpu
+def test_gated_weight_gradients_of_very_many_rows():
+    """Sums over 100 million rows, of one sign.  u and du are 1 (x's first column times the first rows of the weights, dh = 1), so that nothing is
+    rounded before the sum.  A chain of CHAIN values loses at most 2^-23 with each of its CHAIN / 16 additions, the join half a step of
+    the running sum with each of at most 64 + parts / 64."""
+    c, m, n = capi(), 100_000_000, 8
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = (torch.rand(m, n, generator=g, device="cuda", dtype=F16) + 1) * 2.0 ** -13
+    x[:, 0] = 1
+    w = torch.zeros(n, n, dtype=F16, device="cuda")
+    w[0] = 1
+    _, _, dwu = c.gated_linear_grad(torch.ones(m, n, dtype=F16, device="cuda"), None, None, x, w, w, "relu", want_dx=False)
+    want = sum(x[a:a + 10_000_000].double().sum(dim=0) for a in range(0, m, 10_000_000))[1:, None].expand(n - 1, n)
+    parts = -(-m // CHAIN)
+    ref.close(dwu[1:], want, (CHAIN / 16 * 2.0 ** -23 + (64 + parts / 64) * 2.0 ** -24) * want, what="dWu")
