@@ -5,9 +5,9 @@
 //   g = dy * w, xhat = r * rstd, dx = dr + rstd * (g - xhat * mean(g * xhat)), dw = sum over rows of dy * xhat.
 //
 // Memory bound.  A row is read once and stays in registers: WPR warps hold it, up to NV steps each (a step is 32 lanes x 16 bytes).  Sums
-// of a row are fp32: at most 32 terms a lane, then a tree over lanes and warps, so an error of a few 2^-24.  (Joining them and taking the
+// of a row are fp32: at most 16 terms a lane, then a tree over lanes and warps, so an error of a few 2^-24.  (Joining them and taking the
 // root in double was the bound of short rows: 600,000 x 256 in bf16 took 251 us forward and 429 us backward.)  Rows too wide for the
-// registers are read twice.
+// registers are read twice, and a lane's terms, up to 32768 of them, are gathered with their rounding errors (Acc), so that the sum is as good.
 #include <algorithm>
 #include <initializer_list>
 
@@ -39,6 +39,9 @@ template <int LPR> __device__ __forceinline__ float row_sum(float v, int wpr, in
   __syncthreads();                                   // s_part may be written again
   return v;
 }
+
+// A sum with its rounding errors; one that has left fp32 has none (infinity less infinity), and stays what it is.
+__device__ __forceinline__ float finite_sum(const Acc &s) { return fabsf(s.hi) <= FLT_MAX ? s.value() : s.hi; }
 
 // NV > 0: the row is held in registers.  NV == 0: any width, the row is read twice.
 template <typename T, typename R, int NV, bool FP8>
@@ -86,14 +89,16 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const NormArgs a) {
       }
     }
   } else {
+    Acc sum{0.f, 0.f};
     for (int step = w0; step < steps; step += a.wpr) {
       const typename R::Raw t = R::raw(x, step, lane, a.n);
       take(t, res ? R::raw(res, step, lane, a.n) : t, step, v[0]);
       float part = 0.f;
 #pragma unroll
       for (int j = 0; j < E; ++j) part = fmaf(v[0][j], v[0][j], part);
-      ss += part;
+      sum.add(part);
     }
+    ss = finite_sum(sum);
   }
   const float rstd = 1.f / sqrtf(row_sum<R::LPR>(ss, a.wpr, warp, lane, s_part) / (float)a.n + a.eps);
   if (a.rstd && w0 == 0 && lane == 0 && live) a.rstd[row] = rstd;
@@ -255,15 +260,15 @@ __global__ void __launch_bounds__(512) rms_norm_grad_wide_kernel(const NormGradA
 #pragma unroll
     for (int j = 0; j < E; ++j) xh[j] *= rstd, g[j] *= w[j];
   };
-  float sum = 0.f;
+  Acc sum{0.f, 0.f};
   for (int step = warp; step < steps; step += a.wpr) {
     read(step);
     float part = 0.f;
 #pragma unroll
     for (int j = 0; j < E; ++j) part = fmaf(g[j], xh[j], part);
-    sum += part;
+    sum.add(part);
   }
-  const float mean = row_sum<32>(sum, a.wpr, warp, lane, s_part) / (float)a.n;
+  const float mean = row_sum<32>(finite_sum(sum), a.wpr, warp, lane, s_part) / (float)a.n;
   for (int step = warp; step < steps; step += a.wpr) {
     read(step);
     float o[E];
@@ -280,12 +285,12 @@ template <typename T>
 __global__ void __launch_bounds__(256) rms_norm_dw_wide_kernel(const NormGradArgs a) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= a.n) return;
-  float s = 0.f;
+  Acc s{0.f, 0.f};
   for (int64_t row = blockIdx.y; row < a.m; row += gridDim.y) {
     const int64_t i = row * a.n + c;
-    s = fmaf(to_float(static_cast<const T *>(a.dy)[i]), to_float(static_cast<const T *>(a.r)[i]) * __ldg(a.rstd + row), s);
+    s.add(to_float(static_cast<const T *>(a.dy)[i]) * (to_float(static_cast<const T *>(a.r)[i]) * __ldg(a.rstd + row)));
   }
-  a.part[(int64_t)blockIdx.y * a.n + c] = s;
+  a.part[(int64_t)blockIdx.y * a.n + c] = finite_sum(s);
 }
 
 // dw = the partial sums' sum, in a fixed order, in double: 32 threads a column, eight loads of each under way (with eight threads a column

@@ -298,3 +298,23 @@ def test_gated_weight_gradients_of_very_many_rows():
     want = sum(x[a:a + 10_000_000].double().sum(dim=0) for a in range(0, m, 10_000_000))[1:, None].expand(n - 1, n)
     parts = -(-m // CHAIN)
     ref.close(dwu[1:], want, (CHAIN / 16 * 2.0 ** -23 + (64 + parts / 64) * 2.0 ** -24) * want, what="dWu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [16400, 1 << 20, 1 << 24])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_norm_of_very_wide_rows(n, dtype):
+    """Equal values: every addition of a running sum rounds the same way."""
+    c = capi()
+    x, dy, w = (torch.full(s, v, device="cuda").to(dtype) for s, v in (((2, n), 1.1), ((2, n), 1.3), ((n,), 0.9)))
+    y, rstd = c.rms_norm(x, w, 0.0, return_rstd=True)
+    _, rstd64, want = ref.rms_norm(x, None, w, 0.0)
+    ref.close(rstd, rstd64[:, 0], ref.FP32 * rstd64[:, 0], what="rstd")
+    ref.close(y, want, ref.FP32 * want, what="y")
+    dx, dw = c.rms_norm_grad(x, w, rstd, dy)
+    want, want_dw, size, size_dw = ref.rms_norm_grad(x, rstd64, w, dy, None)
+    ref.close(dx, want, ref.FP32 * size, what="dx")
+    ref.close(dw, want_dw, ref.FP32 * size_dw, what="dw")
+    q = c.rms_norm_fp8(x, w, 0.0)
+    want, _ = ref.quantize_rows(ref.rms_norm(x, None, w, 0.0)[2])
+    assert torch.equal(ref.rows_value(q), want)
