@@ -149,9 +149,7 @@ __device__ __forceinline__ int fp8_exponent(float amax) {
   const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
   return max(e, -126);
 }
-__device__ __forceinline__ float pow2f(int e) {      // -149 <= e <= 127
-  return e >= -126 ? __uint_as_float((uint32_t)(e + 127) << 23) : __uint_as_float(1u << (e + 149));
-}
+__device__ __forceinline__ float pow2f(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
 // What counts towards a block's largest magnitude: non-finite values do not (they become NaN codes by themselves).
 __device__ __forceinline__ float finite_abs(float v) {
   const float a = fabsf(v);
