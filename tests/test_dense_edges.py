@@ -318,3 +318,67 @@ def test_norm_of_very_wide_rows(n, dtype):
     q = c.rms_norm_fp8(x, w, 0.0)
     want, _ = ref.quantize_rows(ref.rms_norm(x, None, w, 0.0)[2])
     assert torch.equal(ref.rows_value(q), want)
+
+
+# ---- refusals, by their reasons ---------------------------------------------------------------------------------------------------
+
+REASONS = {
+    "norm: width": r"rows \(m, n\) and a weight", "norm: residual's shape": "residual must have", "norm: residual's type": "residual must have",
+    "norm: weight's type": "weight must have", "norm: integers": "rows must be float32", "norm: negative eps": "eps must not", "norm: strided rows": "contiguous",
+    "norm8: width": r"rows \(m, n\) and a weight", "norm grad: rstd": "rstd must hold", "norm grad: dy": "gradients must have",
+    "quantize: dimensions": "quantize_fp8 needs rows", "quantize: doubles": "rows must be float32", "quantize weight: dimensions": r"needs \(k, n\) or",
+    "dequantize: output type": "output must be float32", "dequantize: scales' shape": "scales of shape",
+    "mm8: inner dimension": "inner dimensions differ", "mm8: rows not 16 bytes apart": "16-byte boundaries", "mm8: values' type": "must be float8_e4m3fn",
+    "mm8: several types, no pointer": "need a type pointer", "mm8: pointer's length": "type pointer must hold", "mm8: pointer's type": "type pointer must hold",
+    "mm8: output type": "output must be float32", "mm8: out's shape": r"out must be \(m, n\)",
+    "gated: activation": "unknown activation", "gated: float32": "bfloat16 or float16", "gated: mixed types": "must have one type",
+    "gated: weights' shapes": r"two weights \(k, f\)", "gated: inner dimension": r"two weights \(k, f\)", "gated: one weight transposed": "or their transposes",
+    "gated: strided rows": "contiguous", "gated grad: dh": "dh must have", "gated grad: g alone": "projections that gated_linear returned",
+    "gated8: several types": r"two weights \(1, f, k\)", "gated8: weights' shapes": r"two weights \(1, f, k\)", "gated8: activation": "unknown activation",
+    "gated8: output type": "output must be float32", "dense norm: width": r"\(\.\.\., n\) and a weight", "dense gated: inner dimension": r"\(\.\.\., k\) and two weights",
+}
+
+
+def refused_calls(device):
+    from test_dense_refusals import calls
+    return calls(device)
+
+
+def test_every_refusal_has_a_reason():
+    assert set(REASONS) == set(refused_calls("cpu"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", sorted(REASONS))
+def test_refused_for_its_reason(what):
+    with pytest.raises(capi().GphlError, match=REASONS[what]):
+        refused_calls("cuda")[what]()
+
+
+OPERATORS = ["norm", "norm grad", "norm8", "quantize", "quantize weight", "dequantize", "mm8", "gated", "gated grad", "gated8", "dense norm", "dense gated"]
+
+
+def good_calls(device):
+    """A call of each operator that nothing is wrong with but, on the CPU, the device."""
+    from graphiler_b200 import dense
+    c = capi()
+    e = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype, device=device)
+    x, v, w, q = e(4, 64), e(64), e(64, 32), c.Fp8Rows(e(4, 64, dtype=torch.uint8).view(F8), e(4, 1, dtype=F32))
+    qw = c.Fp8Weight(e(1, 32, 64, dtype=torch.uint8).view(F8), e(1, 1, 1, dtype=F32))
+    return dict(zip(OPERATORS, [
+        lambda: c.rms_norm(x, v), lambda: c.rms_norm_grad(x, v, e(4, dtype=F32), x), lambda: c.rms_norm_fp8(x, v), lambda: c.quantize_fp8(x),
+        lambda: c.quantize_fp8_weight(w), lambda: c.dequantize_fp8(q), lambda: c.segment_mm_fp8(q, qw), lambda: c.gated_linear(x, w, w),
+        lambda: c.gated_linear_grad(e(4, 32), None, None, x, w, w), lambda: c.gated_linear_fp8(q, qw, qw), lambda: dense.rms_norm(x, v),
+        lambda: dense.gated_linear(x, w, w)]))
+
+
+@pytest.mark.parametrize("what", OPERATORS)
+def test_no_cpu_path(what):
+    with pytest.raises(capi().GphlError, match="need CUDA tensors"):
+        good_calls("cpu")[what]()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", OPERATORS)
+def test_the_same_call_on_the_gpu(what):
+    good_calls("cuda")[what]()
