@@ -164,10 +164,11 @@ def hgt_layer(pg: PreparedGraph, h, p: Dict[str, torch.Tensor], heads: int, sqrt
 
 
 def feed_forward_layer(h, p: Dict[str, torch.Tensor], residual=None, eps: float = 1e-6, activation: str = "silu"):
-    """Pre-norm gated feed-forward of a graph transformer on the node rows, after its attention layer (``hgt_layer``): with r = h (+
-    ``residual``, e.g. the attention's input), returns ``r + (act(n Wg) * (n Wu)) Wd`` for ``n = rms_norm(r)``.  bfloat16 or float16 rows,
-    differentiable: norm and gated product are one autograd node each; the product back is plain cuBLAS, as the other dense projections.
-    ``p``: norm_weight (d), gate_weight and up_weight (d, f), down_weight (f, d)."""
+    """Pre-norm gated feed-forward of a graph transformer on the node rows, after its attention layer: with r = h (+ ``residual``, e.g. the
+    attention's input), returns ``r + (act(n Wg) * (n Wu)) Wd`` for ``n = rms_norm(r)``.  bfloat16 or float16 rows (..., d), differentiable;
+    ``hgt_layer`` puts out float32, which the caller casts.  Norm and gated product are one autograd node each; the product back is plain
+    cuBLAS, as the other dense projections, and the sum an addition behind it.  ``p``: norm_weight (d), gate_weight and up_weight (d, f),
+    down_weight (f, d)."""
     n = dense.rms_norm(h, p["norm_weight"], eps, residual=residual)
     n, r = (n, h) if residual is None else n
     return r + torch.matmul(dense.gated_linear(n, p["gate_weight"], p["up_weight"], activation), p["down_weight"])

@@ -382,3 +382,34 @@ def test_no_cpu_path(what):
 @pytest.mark.parametrize("what", OPERATORS)
 def test_the_same_call_on_the_gpu(what):
     good_calls("cuda")[what]()
+
+
+# ---- after an attention layer -------------------------------------------------------------------------------------------------------
+
+def block(r, p, rows=lambda v: v, weight=lambda w: w.double()):
+    """r + (silu(n Wg) * (n Wu)) Wd in 64 bits; `rows` and `weight`: what is rounded on the way."""
+    n = rows(ref.rms_norm(r, None, p["norm_weight"], 1e-6)[2])
+    g, u = n @ weight(p["gate_weight"]), n @ weight(p["up_weight"])
+    return r.double() + rows(ref.act(g, "silu")[0] * u) @ weight(p["down_weight"])
+
+
+@pytest.mark.gpu
+def test_feed_forward_after_attention():
+    """The attention layer puts out 32 bits: the 8-bit form takes them, the 16-bit form takes them cast and refuses them as they are."""
+    from graphiler_b200 import layers, synthetic
+    w = synthetic.make_c4(scale=0.01).to("cuda")
+    a = layers.hgt_layer(layers.PreparedGraph(w.graph), w.feats, w.params, int(w.hyper["heads"]), w.hyper["sqrt_dk"])
+    d = a.shape[1]
+    p = ff_params(d, 3 * d + 8)
+    with pytest.raises(capi().GphlError, match="type|bfloat16"):
+        layers.feed_forward_layer(a, {k: v.float() for k, v in p.items()})
+    h = a.bfloat16()
+    got, want = layers.feed_forward_layer(h, p), block(h, p)
+    # n, the gated rows, the product and the sum are rounded once each: four half steps of the largest value, and as much for what the products add up
+    assert float((got.double() - want).abs().max()) <= 8 * ref.half_step(BF16) * float(want.abs().max())
+    p32 = {k: v.float() for k, v in p.items()}
+    got = layers.feed_forward_layer_fp8(a, layers.prepare_feed_forward_fp8(p32))
+    want = block(a, p32, rows=lambda v: ref.quantize_rows(v)[0], weight=lambda w: ref.quantize_weight(w[None])[0][0].t())
+    assert got.dtype == F32
+    # codes beside a border fall on its other side for a share of 2^-16 of n, which moves g and u by 2^-11 and a share of 2^-7 of the second codes by 2^-3
+    assert float((got.double() - want).norm()) <= 2.0 ** -6.5 * float((want - a.double()).norm()) + 2 * ref.half_step(F32) * float(want.norm())
