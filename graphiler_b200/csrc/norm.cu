@@ -379,10 +379,11 @@ template <typename T, typename R> static void grad_launch(NormGradArgs a, int sm
   g = grad_shape(a.m, a.n, R::E, R::LPR, sms);
   a.wpr = g.wpr;
   if (g.wpr > 0) {
-    // 64 registers a thread are enough for 16-bit rows; fp32 rows and single columns spill with them and get up to 128 (and fewer warps) while
-    // blocks are small enough
-    if (R::E == 4 && g.warps <= 16) rms_norm_grad_kernel<T, R, 512><<<g.grid, g.warps * 32, g.smem, s>>>(a);
-    else rms_norm_grad_kernel<T, R, 1024><<<g.grid, g.warps * 32, g.smem, s>>>(a);
+    // Whole vectors of 16-bit rows do with 64 registers a thread (8 to 12 bytes of them spill).  fp32 rows and single columns would spill 104 to 136
+    // bytes: they get up to 128 registers, and fewer warps, while 16 warps hold a row (4096 values), and spill beyond.
+    if constexpr (R::E == 8 || R::LPR == 32)
+      if (R::E == 8 || g.warps > 16) return rms_norm_grad_kernel<T, R, 1024><<<g.grid, g.warps * 32, g.smem, s>>>(a);
+    if constexpr (R::E == 4) rms_norm_grad_kernel<T, R, 512><<<g.grid, g.warps * 32, g.smem, s>>>(a);
   } else if constexpr (R::LPR == 32) {
     a.wpr = 16;
     // dw's parts first: dx may lie over dy
