@@ -655,9 +655,10 @@ def segment_mm_fp8(x: Fp8Rows, w: Fp8Weight, type_pointer=None, out_dtype=torch.
 
 
 def gated_linear(x, w_gate, w_up, activation: str = "silu", return_projections: bool = False):
-    """Gated feed-forward ``act(x @ w_gate) * (x @ w_up)`` in one kernel; ``activation``: silu, gelu (the exact form) or relu.  bfloat16 or
-    float16 rows (m, k) and weights (k, f), each contiguous, or both weights transposed views of contiguous (f, k) tensors; sums in
-    float32.  With ``return_projections``: (h, g, u), the two products in float32 with rows padded to a multiple of 4 columns, for
+    """Gated feed-forward ``act(x @ w_gate) * (x @ w_up)`` in one kernel (and one that joins parts, where k is split for want of tiles);
+    ``activation``: silu, gelu (the exact form) or relu.  bfloat16 or float16 rows (m, k) and weights (k, f), each contiguous, or both weights
+    transposed views of contiguous (f, k) tensors; sums in float32.  Rows of a width that is no multiple of 8 are copied to padded ones in
+    every call, weights included: with few rows of x that costs more than the product.  With ``return_projections``: (h, g, u), the two products in float32 with rows padded to a multiple of 4 columns, for
     ``gated_linear_grad``.  No gradients are recorded: see ``graphiler_b200.dense``."""
     out = _call("gated_linear_rows", x, w_gate, w_up, activation, return_projections)
     return tuple(out) if return_projections else out[0]
@@ -665,7 +666,8 @@ def gated_linear(x, w_gate, w_up, activation: str = "silu", return_projections: 
 
 def gated_linear_grad(dh, g, u, x, w_gate, w_up, activation: str = "silu", want_dx: bool = True, want_dw: bool = True):
     """Gradients of ``gated_linear``: (dx, dw_gate, dw_up), the weights' laid out as the weights; None where not wanted.  ``g``, ``u``: the
-    projections that ``gated_linear`` returned, or None: they are made again."""
+    projections that ``gated_linear`` returned, or None: they are made again.  The projections' own gradients are rounded to the rows' type
+    between the products (in float16 those beyond 65504 become infinite)."""
     out = _call("gated_linear_grad", dh, g, u, x, w_gate, w_up, activation, want_dx, want_dw)
     dx = out[0] if want_dx else None
     return (dx,) + (tuple(out[-2:]) if want_dw else (None, None))

@@ -1,8 +1,8 @@
 // The tensor-core product of the dense operators for sm_100a: out[i, j] = sum_k A[i, k] B[j, k], 16-bit or e4m3 operands, fp32 sums.
 //
-// One persistent block per SM, or one pair of blocks per two SMs, walks tiles of 128 (256) rows x BN columns of the output.  Ten warps: one brings boxes of A and B into a ring of
+// One persistent block per SM, or one pair of blocks per two SMs, walks tiles of 128 (256) rows x BN columns of the output.  One warp brings boxes of A and B into a ring of
 // shared-memory stages by TMA (128 bytes of k per stage, 128-byte swizzle), one issues tcgen05.mma into one of two accumulators in
-// TMEM, eight read the other one back and finish the tile, so that loads, products and stores of neighbouring tiles overlap.
+// TMEM, eight or sixteen read the other one back and finish the tile, so that loads, products and stores of neighbouring tiles overlap.
 // 16-bit: an accumulator gathers a whole tile.  e4m3: it holds one block of 128 k, which the eight warps scale (row scale x weight
 // scale) and add to fp32 registers: the scales may differ from block to block, and no sum outlives a block inside the tensor core.
 // GATED tiles multiply the same rows by BN/2 columns of each of two weights; both halves of the accumulator meet in the epilogue.
@@ -961,8 +961,8 @@ template <int BN, int CTAS, int EPI_WARPS, bool FP8, int MODE> static int run(co
   return launched("gemm_kernel");
 }
 template <bool FP8, int MODE> static int run_shape(const Shape &s, const GemmArgs &a, int sms, cudaStream_t stream) {
-  // 16 epilogue warps where they have an activation to compute, 8 where they only store (300,000 x 256 -> 1024: 337 against 391 us when that was measured, 321 now) or
-  // hold sums
+  // 16 epilogue warps where they have an activation to compute (300,000 x 256 -> 1024 forward: 337 us, with 8 warps 391, an element at a time; 320 since
+  // silu takes two), 8 where they only store or hold sums
   constexpr int WARPS = FP8 || MODE == LINEAR ? 8 : 16;
   if (s.ctas == 2) return run<256, 2, WARPS, FP8, MODE>(a, sms, stream);
   if (s.bn == 256) return run<256, 1, WARPS, FP8, MODE>(a, sms, stream);

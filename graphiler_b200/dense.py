@@ -20,5 +20,6 @@ def rms_norm(x, weight, eps: float = 1e-6, residual=None):
 
 def gated_linear(x, w_gate, w_up, activation: str = "silu"):
     """``capi.gated_linear`` on (..., k) with gradients of x and both weights.  Kept for the backward pass: the inputs and, for rows
-    wider than 768, the two projections in float32 (8 bytes per element of the output); narrower rows make them again."""
+    wider than 768, the two projections in float32 (8 bytes per element of the output); narrower rows make them again.  The projections'
+    gradients are rounded to the rows' type on the way, with its range."""
     return _call("gated_linear", x, w_gate, w_up, activation)

@@ -306,7 +306,8 @@ int gphl_debug_reset_wait_timeouts(void); /* sets the counter back to 0 (synchro
 
 /* r = round(x + residual) in the rows' type (r = x without a residual; then r may be NULL), y = r * rstd * w with
  * rstd = 1 / sqrt(mean(r^2) + eps).  (m, n) row-major, m rows < 2^31; w: n values of the rows' type or fp32.  rstd (m, may be NULL) is
- * kept for the backward pass.  y may be x, r may be x or residual. */
+ * kept for the backward pass.  y may be x, r may be x or residual.  Squares are summed in fp32: a row
+ * whose sum leaves it (values of about 1e19) becomes 0. */
 int gphl_rms_norm(int32_t dtype, int64_t m, int64_t n, const void *x, const void *residual, const void *w, int32_t w_dtype, float eps,
                   void *y, void *r, float *rstd, void *stream);
 /* The same with y as codes (rounded once, from the fp32 value). */
@@ -341,13 +342,15 @@ int gphl_segment_mm_fp8(int64_t n_types, const int32_t *type_pointer, int64_t m,
                         const float *x_scales, int64_t scale_row_stride, int64_t scale_block_stride, const void *w, int64_t w_stride,
                         const float *w_scales, int32_t out_dtype, void *y, void *workspace, void *stream);
 
-/* Gated feed-forward h = act(x Wg) * (x Wu), both projections, the activation and the product in one kernel.  x (m, k), row stride ldx;
+/* Gated feed-forward h = act(x Wg) * (x Wu), both projections, the activation and the product in one kernel (few tiles, or k beyond 32768: k is
+ * split, and a second kernel joins the parts).  x (m, k), row stride ldx;
  * weights (k, f) with row stride ldw, or, `w_transposed`, (f, k) with row stride ldw; h (m, f) contiguous; dtype bf16 or fp16, sums
  * fp32.  g, u (both or neither): the two projections in fp32, row stride ld_gu (a multiple of 4), for the backward pass. */
 int64_t gphl_gated_workspace_bytes(int64_t m, int64_t k, int64_t f);
 int gphl_gated(int32_t dtype, int32_t act, int64_t m, int64_t k, int64_t f, const void *x, int64_t ldx, const void *wg, const void *wu,
                int64_t ldw, int32_t w_transposed, void *h, float *g, float *u, int64_t ld_gu, void *workspace, void *stream);
-/* Its backward pass: dg = dh u act'(g), du = dh act(g) (rounded to dtype), dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du.
+/* Its backward pass: dg = dh u act'(g), du = dh act(g), dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du.  dg and du are rounded to dtype
+ * between the products, and take its range: in fp16 one beyond 65504 is infinite, and so is what it reaches (scale dh so that it is not).
  * g and u as gphl_gated stored them, or both NULL: they are made again from x and the weights.
  * dx (m, k) and dWg, dWu (laid out as the weights, contiguous) may each be NULL when not wanted (the two weights' together). */
 int64_t gphl_gated_grad_workspace_bytes(int64_t m, int64_t k, int64_t f);
