@@ -413,3 +413,61 @@ def test_feed_forward_after_attention():
     assert got.dtype == F32
     # codes beside a border fall on its other side for a share of 2^-16 of n, which moves g and u by 2^-11 and a share of 2^-7 of the second codes by 2^-3
     assert float((got.double() - want).norm()) <= 2.0 ** -6.5 * float((want - a.double()).norm()) + 2 * ref.half_step(F32) * float(want.norm())
+
+
+# ---- offsets beyond 32 bits -----------------------------------------------------------------------------------------------------------
+
+BLOCK_ROWS, REPS, FAR = 656, 400, 8200            # 262,400 rows of 8200: 2.15e9 values
+
+
+def repeated(*shape, seed, dtype=BF16):
+    """A block of rows, again and again: every block has to come out as the first one does."""
+    return randn(BLOCK_ROWS, *shape, seed=seed, dtype=dtype).repeat(REPS, 1)
+
+
+def blocks_alike(y):
+    first = y[:BLOCK_ROWS]
+    return all(torch.equal(y[a:a + BLOCK_ROWS], first) for a in range(0, y.shape[0], BLOCK_ROWS))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [FAR, FAR + 1])
+def test_norms_of_far_rows(n):
+    c = capi()
+    x, res, w = repeated(n, seed=1), repeated(n, seed=2), randn(n, seed=3, dtype=BF16)
+    y, r, rstd = c.rms_norm(x, w, residual=res, return_rstd=True)
+    assert blocks_alike(y) and blocks_alike(r) and blocks_alike(rstd)
+    _, _, want = ref.rms_norm(x[:8], res[:8], w, 1e-6)
+    ref.close(y[:8], want, ref.FP32 * want.abs())
+    dx, dw = c.rms_norm_grad(r, w, rstd, y, res)
+    assert blocks_alike(dx) and torch.isfinite(dw).all()
+    del dx, y, r
+    q, r = c.rms_norm_fp8(x, w, residual=res)
+    assert blocks_alike(q.values.view(torch.uint8)) and blocks_alike(q.scales) and blocks_alike(r)
+    del q, r, res
+    q = c.quantize_fp8(x)
+    assert blocks_alike(q.values.view(torch.uint8)) and blocks_alike(q.scales)
+    assert blocks_alike(c.dequantize_fp8(q, BF16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [FAR, FAR + 1])
+def test_products_of_far_rows(n):
+    c = capi()
+    x, w = repeated(128, seed=1), randn(128, n, seed=2, dtype=BF16)
+    x8, w8 = c.quantize_fp8(x), c.quantize_fp8_weight(w)
+    y = c.segment_mm_fp8(x8, w8)
+    assert blocks_alike(y)
+    want = ref.rows_value(x8)[:8] @ ref.weight_value(w8)[0].t()
+    ref.close(y[:8], want, ref.sum_loss(128, fp8=True) * (ref.rows_value(x8)[:8].abs() @ ref.weight_value(w8)[0].t().abs()))
+    del y
+    q = c.gated_linear_fp8(x8, w8, w8)
+    assert blocks_alike(q.values.view(torch.uint8)) and blocks_alike(q.scales)
+    del q
+    h, g, u = c.gated_linear(x, w, w, return_projections=True)
+    assert blocks_alike(h) and blocks_alike(g[:, :n]) and blocks_alike(u[:, :n])
+    dx, _, _ = c.gated_linear_grad(h, g, u, x, w, w)
+    assert blocks_alike(dx)
+    del g, u
+    again, _, _ = c.gated_linear_grad(h, None, None, x, w, w)
+    assert torch.equal(again, dx)
